@@ -13,6 +13,7 @@ import os
 import torch
 
 from tinyserve_llm_b200.ops.build import build_library
+from tinyserve_llm_b200.ops.microscaled import MXFP4
 
 _DTYPE_CODE = {torch.float32: 0, torch.bfloat16: 1}
 
@@ -107,6 +108,9 @@ _SIGNATURES = {
     "ts_row_scaled_activation": ("int", "ppppiiiip"),
     "ts_difference_head_norm": ("int", "plipl" "piiii" "fffip"),
     "ts_scale_tanh_cap": ("int", "plffp"),
+    "ts_quantize_mxfp4": ("int", "ppplilllip"),
+    "ts_dequantize_mxfp4": ("int", "ppplillip"),
+    "ts_gemm_mxfp4": ("int", "ppllplplp" "iiil" "iiffipp"),
 }
 _CTYPES = {"p": ctypes.c_void_p, "i": ctypes.c_int, "l": ctypes.c_longlong, "f": ctypes.c_float}
 _RETURNS = {"int": ctypes.c_int, "long long": ctypes.c_longlong, "void": None, "const char*": ctypes.c_char_p}
@@ -137,6 +141,12 @@ _WAIT_CODES: dict[int, tuple[str, str]] = {
     27: ("sgemm_tcgen05", "TMA producer of x waiting for a free operand tile"),
     31: ("delta_tiles", "warps of the state waiting for a tile"),
     32: ("delta_tiles", "warps of U and the output waiting for a tile"),
+    41: ("gemm_mxfp4", "TMA producer waiting for a free ring slot"),
+    42: ("gemm_mxfp4", "MMA issuer waiting for operands"),
+    43: ("gemm_mxfp4", "epilogue waiting for an accumulator"),
+    44: ("gemm_mxfp4", "MMA issuer waiting for a drained accumulator"),
+    45: ("gemm_mxfp4", "warps of the scales waiting for a free ring slot"),
+    46: ("gemm_mxfp4", "warps that spread codes waiting for a free ring slot"),
 }
 
 
@@ -1654,6 +1664,98 @@ class Ops:
         if out_dtype != x.dtype:
             return torch.mm(x, weight.t(), out_dtype=out_dtype, out=out)
         return torch.mm(x, weight.t(), out=out)
+
+    # ------------------------------------------------------------------ microscaled 4-bit floating point
+    @staticmethod
+    def _check_here(device: torch.device, name: str) -> None:
+        """The kernels run on the current device's current stream: what they read has to lie there."""
+        if device.type != "cuda":
+            raise KernelError(f"{name} must be on a CUDA device; the engine has no CPU path")
+        if device.index is not None and device.index != torch.cuda.current_device():
+            raise KernelError(f"{name} is on {device}, the current device is cuda:{torch.cuda.current_device()}")
+
+    def quantize_mxfp4(self, x: torch.Tensor) -> MXFP4:
+        """
+        The rows of x (float32 or bfloat16 [rows, cols], any number of columns, rows may be stretches of wider rows) in microscaled 4-bit
+        floating point: of a block of 32 numbers with largest magnitude a, the scale is 2^(floor(log2 a) - 2), at least 2^-127, and a code
+        the nearest to x / scale, ties to the even code, magnitudes over 6 to 6.  A block that holds an infinity or a NaN becomes NaN.
+        """
+        if x.dim() != 2 or x.dtype not in _DTYPE_CODE or (x.shape[1] > 1 and x.stride(1) != 1):
+            raise KernelError(f"quantize_mxfp4: x must be a [rows, columns] stretch of float32 or bfloat16, got {x.dtype} {tuple(x.shape)}")
+        rows, cols = x.shape
+        if cols == 0:
+            raise KernelError("quantize_mxfp4: x has no columns")
+        self._check_here(x.device, "x")
+        q = MXFP4.empty(rows, cols, x.device)
+        if rows:
+            self._call("ts_quantize_mxfp4", _ptr(x), _ptr(q.codes), _ptr(q.scales), rows, cols, x.stride(0) if rows > 1 else cols, q.ld_codes,
+                       q.ld_scales, _DTYPE_CODE[x.dtype], _stream())
+        return q
+
+    def dequantize_mxfp4(self, q: MXFP4, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+        """The numbers q stands for, [rows, cols] in bfloat16 or float32: exact, but for what the type has no room for (infinite)."""
+        if dtype not in _DTYPE_CODE:
+            raise KernelError(f"dequantize_mxfp4: dtype {dtype}, expected one of {tuple(_DTYPE_CODE)}")
+        self._check_here(q.device, "q")
+        out = torch.empty((q.rows, q.cols), dtype=dtype, device=q.device)
+        if q.rows:
+            self._call("ts_dequantize_mxfp4", _ptr(q.codes), _ptr(q.scales), _ptr(out), q.rows, q.cols, q.ld_codes, q.ld_scales,
+                       _DTYPE_CODE[dtype], _stream())
+        return out
+
+    def linear_mxfp4(self, x: torch.Tensor | MXFP4, weight: MXFP4, out_dtype: torch.dtype | None = None,
+                     out: torch.Tensor | None = None) -> torch.Tensor:
+        """
+        x . weight^T, [M, N] in bfloat16 (or `out_dtype` float32), with the weight's rows in microscaled 4-bit floating point.  x: bfloat16
+        [M, K], K a multiple of 8, rows contiguous or stretches of wider rows that start 16-byte aligned; or rows quantised like the weight
+        (any K): then both sides stay in four bits.  Sums in float32, rounded once.  `out` (contiguous, of the output dtype) receives the product.
+        """
+        out_dtype = out_dtype or torch.bfloat16
+        if out_dtype not in _DTYPE_CODE:
+            raise KernelError(f"linear_mxfp4: output dtype {out_dtype}, expected one of {tuple(_DTYPE_CODE)}")
+        return self._product_mxfp4("linear_mxfp4", x, weight, None, 0.0, 1.0, out_dtype, out)
+
+    def linear_gated_mxfp4(self, x: torch.Tensor | MXFP4, gate_up_weight: MXFP4, activation: str, limit: float = 0.0,
+                           alpha: float = 1.0) -> torch.Tensor:
+        """
+        act(x . Wgate^T, x . Wup^T), bfloat16 [M, I], for the activations of `gated_activation` and x as `linear_mxfp4` takes it; Wgate and
+        Wup are the two halves of the weight's rows.  The activation reads the float32 sums: one rounding, at the end.
+        """
+        if gate_up_weight.rows % 2 or activation not in self.GATED_ACTIVATIONS:
+            raise KernelError(f"linear_gated_mxfp4: the weight must hold gate and up halves ({gate_up_weight.rows} rows); activation "
+                              f"{activation!r} of {sorted(self.GATED_ACTIVATIONS)}")
+        return self._product_mxfp4("linear_gated_mxfp4", x, gate_up_weight, activation, limit, alpha, torch.bfloat16, None)
+
+    def _product_mxfp4(self, who: str, x: torch.Tensor | MXFP4, w: MXFP4, activation: str | None, limit: float, alpha: float,
+                       out_dtype: torch.dtype, out: torch.Tensor | None) -> torch.Tensor:
+        both = isinstance(x, MXFP4)
+        M, K = (x.rows, x.cols) if both else tuple(x.shape) if x.dim() == 2 else (-1, -1)
+        if M < 0 or K != w.cols:
+            raise KernelError(f"{who}: x is {tuple(x.codes.shape if both else x.shape)}, the weight has rows of {w.cols} numbers")
+        self._check_here(w.device, "weight")
+        self._check_here(x.device, "x")
+        if not both:
+            if x.dtype != torch.bfloat16:
+                raise KernelError(f"{who}: x has dtype {x.dtype}; the products over 4-bit weights take bfloat16 or quantised rows")
+            ldx = x.stride(0) if M > 1 else K
+            if K % 8 or (K > 1 and x.stride(1) != 1) or ldx % 8 or ldx < K or x.data_ptr() % 16:
+                raise KernelError(f"{who}: x must have a multiple of 8 columns, contiguous, in rows that start 16-byte aligned "
+                                  f"(shape {tuple(x.shape)}, strides {x.stride()})")
+        cols = w.rows if activation is None else w.rows // 2
+        if out is None:
+            out = torch.empty((M, cols), dtype=out_dtype, device=w.device)
+        else:
+            self._check(out, "out", out_dtype, 2)
+            self._check_here(out.device, "out")
+            if tuple(out.shape) != (M, cols):
+                raise KernelError(f"{who}: out is {tuple(out.shape)}, the product {(M, cols)}")
+        if M == 0 or cols == 0:
+            return out
+        kind = 0 if activation is None else self.GATED_ACTIVATIONS[activation]
+        self._call("ts_gemm_mxfp4", _ptr(w.codes), _ptr(w.scales), w.ld_codes, w.ld_scales, _ptr(x.codes) if both else _ptr(x),
+                   x.ld_codes if both else ldx, _ptr(x.scales) if both else 0, x.ld_scales if both else 0, _ptr(out), M, w.rows, K, cols,
+                   0 if activation is None else 1, kind, limit, alpha, _DTYPE_CODE[out_dtype], self.error_word().data_ptr(), _stream())
+        return out
 
     def linear_columns(self, x: torch.Tensor, weight: torch.Tensor, out_dtype: torch.dtype | None = None) -> torch.Tensor:
         """
