@@ -1,0 +1,300 @@
+// What the products y = x . W^T with W in microscaled 4-bit floating point (mxfp4.cuh) share on the fifth-generation tensor cores:
+// gemm_mxfp4_rows16.cu takes rows of x in bfloat16, gemm_mxfp4_rows4.cu rows in four bits too.
+//
+// W's rows are the M of the MMA, 128 a tile, and x's rows its N (BN: 32 to 256), so that a few rows of x cost an MMA of few columns and
+// not one of 128 rows: accumulator lane = row of W, column = row of x.  K goes by chunks of 256 numbers, 128 bytes of codes a row.
+//
+// Gated (y = act(x Wgate^T, x Wup^T), W = [gate rows | up rows]): a tile holds 16 gate rows, the 16 up rows that belong to them, and so
+// on, so that a gate lies 16 lanes before its up in the same warp's quarter of tensor memory and one shuffle brings them together.
+//
+// Many tiles: persistent, one CTA an SM, two accumulators, so that a tile's epilogue runs under the next one's MMAs.  Few tiles: a cluster
+// of `splits` CTAs takes a tile, each its share of K, and leaves its sums in its own shared memory; each CTA then adds up a share of the
+// columns from all of them, in the order of their ranks.  Nothing of that needs a workspace in global memory, and the order is fixed.
+//
+// Every wait on an mbarrier gives up after about two seconds, records where in an error word the host can read, and the CTA goes on to
+// free its tensor memory and return.
+#pragma once
+
+#include "mxfp4.cuh"
+#include "tcgen05.cuh"
+
+struct MxParams {
+    const uint8_t* w_codes;
+    const uint8_t* w_scales;
+    long long w_ld_codes, w_ld_scales;
+    const uint8_t* x_scales;                           // rows in four bits
+    long long x_ld_scales;
+    void* y;
+    long long ldy;
+    int M, N, K, blocks;                               // rows of x, rows of W, columns, blocks of 32 of them
+    int inter;                                         // gated: rows of W per half
+    int out_f32, act;
+    float act_limit, act_alpha;
+    int one_box;                                       // gated: a tile's codes are one box of a map of four dimensions
+    int settled;                                       // W may be read before the kernels ahead on the stream have finished
+    int splits;
+    int* error;
+};
+
+// Either form's products: the launcher's checks have been made.
+int mxfp4_rows16(const void* x, long long ldx, MxParams& p, int gated, cudaStream_t stream);
+int mxfp4_rows4(const void* x, long long ldx, MxParams& p, int gated, cudaStream_t stream);
+
+namespace {
+
+constexpr int BM = 128, ROW = 128, CHUNK = 256;       // rows of W a tile; bytes of a row of codes (or of a stage); numbers they hold
+constexpr int A_BYTES = BM * ROW;
+
+// A bounded wait whose first look costs no clock: between MMAs of few columns the issuer's own instructions are what takes the time.
+__device__ __forceinline__ bool wait_for(uint64_t* bar, uint32_t parity, int* error, int code) {
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(done) : "r"(smem_u32(bar)), "r"(parity) : "memory");
+    return done ? true : mbar_wait(bar, parity, error, code);
+}
+// A place in a ring of SIZE barriers and the parity of its round.
+template <int SIZE>
+struct Ring {
+    int at = 0;
+    uint32_t parity = 0;
+    __device__ __forceinline__ void next() {
+        if (++at == SIZE) at = 0, parity ^= 1;
+    }
+};
+
+__device__ __forceinline__ void tma_load_4d(void* smem, const CUtensorMap* map, uint64_t* bar, int x, int y, int z, int w) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
+        ::"r"(smem_u32(smem)), "l"(map), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
+}
+
+__device__ __forceinline__ void tmem_ld16(uint32_t addr, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+          "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(addr) : "memory");
+}
+
+// The activation is chosen once for many values, so that what runs is one short loop and not four activations in a row.
+template <int ACT>
+__device__ __forceinline__ float gated_value(const MxParams& p, float g, float u) {
+    if (ACT == TS_ACT_SILU) return __fdividef(g, 1.f + __expf(-g)) * u;
+    return ts_gated_activation(ACT, g, u, p.act_limit, p.act_alpha);
+}
+template <int ACT>
+__device__ __forceinline__ void gate_eight(const MxParams& p, float (&v)[8], const float (&u)[8]) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = gated_value<ACT>(p, v[j], u[j]);
+}
+__device__ __forceinline__ float gate_one(const MxParams& p, float g, float u) {
+    if (p.act == TS_ACT_SILU) return gated_value<TS_ACT_SILU>(p, g, u);
+    return ts_gated_activation(p.act, g, u, p.act_limit, p.act_alpha);
+}
+
+// The row of W in lane l of a tile whose first output column is f0.
+template <bool GATED>
+__device__ __forceinline__ int row_of(const MxParams& p, int f0, int l) {
+    if (!GATED) return f0 + l;
+    return f0 + (l >> 5) * 16 + (l & 15) + ((l & 16) ? p.inter : 0);
+}
+
+__host__ __device__ constexpr int power_of_two(int n) { return n <= 32 ? 32 : n <= 64 ? 64 : n <= 128 ? 128 : n <= 256 ? 256 : 512; }
+
+// Sixteen columns of a warp's quarter: column c of the accumulator is row t0 + c of x.  `f`: this lane's output column.
+template <bool GATED>
+__device__ __forceinline__ void store_sixteen(const MxParams& p, const uint32_t (&acc)[16], int t, int f, int outs, bool paired, int lane) {
+    if (GATED) {
+        float v[8], u[8];                            // the lower half of the lanes finishes columns 0, 2, ..., the upper one 1, 3, ...
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float a = __uint_as_float(acc[2 * j]), b = __uint_as_float(acc[2 * j + 1]);
+            const float other = __shfl_xor_sync(0xffffffffu, lane < 16 ? b : a, 16);
+            v[j] = lane < 16 ? a : other;
+            u[j] = lane < 16 ? other : b;
+        }
+        if (p.act == TS_ACT_SILU) gate_eight<TS_ACT_SILU>(p, v, u);
+        else if (p.act == TS_ACT_RELU) gate_eight<TS_ACT_RELU>(p, v, u);
+        else if (p.act == TS_ACT_CLAMPED_SWISH) gate_eight<TS_ACT_CLAMPED_SWISH>(p, v, u);
+        else gate_eight<TS_ACT_GELU_TANH>(p, v, u);
+        t += lane >> 4;
+        __nv_bfloat16* out = (__nv_bfloat16*)p.y + (long long)t * p.ldy + f;
+        if (paired) {                                // neighbours swap: an even lane stores both outputs of one row, an odd one of the other
+#pragma unroll
+            for (int j = 0; j < 8; j += 2) {
+                const float other = __shfl_xor_sync(0xffffffffu, lane & 1 ? v[j] : v[j + 1], 1);
+                const __nv_bfloat162 two = lane & 1 ? __floats2bfloat162_rn(other, v[j + 1]) : __floats2bfloat162_rn(v[j], other);
+                const int jj = 2 * (j + (lane & 1));
+                if (t + jj < p.M && f < outs) *reinterpret_cast<__nv_bfloat162*>(out + (long long)jj * p.ldy - (lane & 1)) = two;
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (t + 2 * j < p.M && f < outs) out[(long long)(2 * j) * p.ldy] = __float2bfloat16_rn(v[j]);
+        }
+    } else if (p.out_f32) {
+        float* out = (float*)p.y + (long long)t * p.ldy + f;
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+            if (t + j < p.M && f < outs) out[(long long)j * p.ldy] = __uint_as_float(acc[j]);
+    } else {
+        __nv_bfloat16* out = (__nv_bfloat16*)p.y + (long long)t * p.ldy + f;
+        if (paired) {
+#pragma unroll
+            for (int j = 0; j < 16; j += 2) {
+                const float a = __uint_as_float(acc[j]), b = __uint_as_float(acc[j + 1]);
+                const float other = __shfl_xor_sync(0xffffffffu, lane & 1 ? a : b, 1);
+                const __nv_bfloat162 two = lane & 1 ? __floats2bfloat162_rn(other, b) : __floats2bfloat162_rn(a, other);
+                const int jj = j + (lane & 1);
+                if (t + jj < p.M && f < outs) *reinterpret_cast<__nv_bfloat162*>(out + (long long)jj * p.ldy - (lane & 1)) = two;
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+                if (t + j < p.M && f < outs) out[(long long)j * p.ldy] = __float2bfloat16_rn(__uint_as_float(acc[j]));
+        }
+    }
+}
+
+// W's codes of a chunk, 128 rows of 128 bytes; gated 16 gate rows, their up rows, and so on, which a map of four dimensions (bytes, 16
+// rows, halves, groups of 16 rows) brings in that order in one box.  Its groups have to be whole: else a box for every 16 rows.
+template <bool GATED>
+__device__ __forceinline__ void load_codes(unsigned char* to, const CUtensorMap* map, uint64_t* bar, const MxParams& p, int chunk, int f0) {
+    if (!GATED) {
+        tma_load_2d(to, map, bar, chunk * ROW, f0);
+    } else if (p.one_box) {
+        tma_load_4d(to, map, bar, chunk * ROW, 0, 0, f0 / 16);
+    } else {
+#pragma unroll
+        for (int g = 0; g < BM / 16; ++g) tma_load_2d(to + g * 16 * ROW, map, bar, chunk * ROW, row_of<true>(p, f0, g * 16));
+    }
+}
+template <bool GATED>
+int make_codes_map(CUtensorMap* map, MxParams& p) {
+    const long long bytes = (long long)p.blocks * 16;
+    if (!GATED || p.inter % 16 || p.inter / 16 < 4) {
+        p.one_box = 0;
+        return make_tile_map(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, p.w_codes, p.N, bytes, p.w_ld_codes, GATED ? 16 : BM, "gemm_mxfp4");
+    }
+    p.one_box = 1;
+    EncodeTiled encode = encode_tiled();
+    if (!encode) return ts_fail("gemm_mxfp4: the driver does not export cuTensorMapEncodeTiled");
+    const cuuint64_t dims[4] = {(cuuint64_t)bytes, 16, 2, (cuuint64_t)p.inter / 16};
+    const cuuint64_t strides[3] = {(cuuint64_t)p.w_ld_codes, (cuuint64_t)p.w_ld_codes * p.inter, (cuuint64_t)p.w_ld_codes * 16};
+    const cuuint32_t box[4] = {ROW, 16, 2, 4}, elem[4] = {1, 1, 1, 1};
+    const CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<uint8_t*>(p.w_codes), dims, strides, box, elem,
+                              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return ts_fail("gemm_mxfp4: cuTensorMapEncodeTiled failed with %d", (int)r);
+    return 0;
+}
+
+// An epilogue warp's share of a tile: columns `first` to `first + SHARE` of the accumulator at `tmem`.  `sums`: where a split tile's go, [column][lane].
+template <bool GATED, int SHARE, bool SPLIT>
+__device__ __forceinline__ void finish_tile(const MxParams& p, uint32_t tmem, int first, int t0, int f0, int outs, bool paired, int quarter, int lane,
+                                            float* sums, uint64_t* drained) {
+    const uint32_t addr = tmem + first + ((uint32_t)(quarter * 32) << 16);
+    const int f = GATED ? f0 + quarter * 16 + (lane & 15) : f0 + quarter * 32 + lane;
+#pragma unroll 1
+    for (int c0 = 0; c0 < SHARE; c0 += 16) {
+        uint32_t acc[16];
+        __syncwarp();
+        tmem_ld16(addr + c0, acc);
+        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+        if (!SPLIT && c0 + 16 == SHARE) {                             // the last of it: the accumulator goes back before the stores
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(drained);
+        }
+        if (SPLIT && p.splits > 1) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) sums[(first + c0 + j) * BM + quarter * 32 + lane] = __uint_as_float(acc[j]);
+        } else if (t0 + first + c0 < p.M) {
+            store_sixteen<GATED>(p, acc, t0 + first + c0, f, outs, paired, lane);
+        }
+    }
+}
+
+// A split tile's share of columns, added up over the cluster's CTAs by `threads` threads, `id` of them this one.
+template <bool GATED>
+__device__ __forceinline__ void join_splits(const MxParams& p, uint32_t sums, int rank, int columns, int t0, int f0, int outs, int id, int threads) {
+    constexpr int OUTS = GATED ? BM / 2 : BM;
+    auto total = [&](int column, int l) {
+        float v = 0.f;
+        for (int r = 0; r < p.splits; ++r) {
+            uint32_t remote;
+            float part;
+            asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(sums + (uint32_t)(column * BM + l) * 4), "r"(r));
+            asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(part) : "r"(remote));
+            v += part;
+        }
+        return v;
+    };
+    const int f = id % OUTS;
+    if (f0 + f >= outs) return;
+    for (int c = rank + p.splits * (id / OUTS); c < columns; c += p.splits * (threads / OUTS)) {
+        const long long at = (long long)(t0 + c) * p.ldy + f0 + f;
+        if (GATED) {
+            const int l = (f >> 4) * 32 + (f & 15);
+            ((__nv_bfloat16*)p.y)[at] = __float2bfloat16_rn(gate_one(p, total(c, l), total(c, l + 16)));
+        } else if (p.out_f32) {
+            ((float*)p.y)[at] = total(c, f);
+        } else {
+            ((__nv_bfloat16*)p.y)[at] = __float2bfloat16_rn(total(c, f));
+        }
+    }
+}
+
+// Launches `kernel` over the tiles: persistent on `sms` SMs, or (`split`) a cluster of p.splits CTAs a tile.
+template <typename Kernel>
+int launch_mxfp4(Kernel kernel, unsigned long long& allowed, int threads, size_t smem, bool split, long long tiles, int sms, int device,
+                 const CUtensorMap& map_w, const CUtensorMap& map_x, const MxParams& p, cudaStream_t stream) {
+    if (device >= 64 || !(allowed >> device & 1)) {                   // a bit a device: what the kernel may ask for is set once on each
+        cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        if (e != cudaSuccess) return ts_fail("gemm_mxfp4: cannot reserve %zu bytes of shared memory: %s", smem, cudaGetErrorString(e));
+        if (device < 64) allowed |= 1ull << device;
+    }
+    TS_REQUIRE(tiles * p.splits <= 0x7fffffffll, "gemm_mxfp4: too many tiles");
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(split ? tiles * p.splits : (tiles < sms ? tiles : sms)));
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    int attrs = 0;
+    if (ts_chaining_enabled()) {
+        attr[attrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[attrs++].val.programmaticStreamSerializationAllowed = 1;
+    }
+    if (p.splits > 1) {
+        attr[attrs].id = cudaLaunchAttributeClusterDimension;
+        attr[attrs].val.clusterDim.x = p.splits;
+        attr[attrs].val.clusterDim.y = 1;
+        attr[attrs++].val.clusterDim.z = 1;
+    }
+    cfg.attrs = attr;
+    cfg.numAttrs = attrs;
+    TS_CHAINED_CHECK("gemm_mxfp4", cudaLaunchKernelEx(&cfg, kernel, map_w, map_x, p));
+    return 0;
+}
+
+// How a product is cut.  run(bn, split) launches tiles of bn rows of x (WIDE, 256, 128, 64, 32).
+template <bool GATED, int WIDE, typename Run>
+int cut_mxfp4(MxParams& p, int sms, const Run& run) {
+    const long long outs = GATED ? p.inter : p.N, per = GATED ? BM / 2 : BM, w_tiles = (outs + per - 1) / per;
+    const int chunks = (p.blocks * MX_BLOCK + CHUNK - 1) / CHUNK;
+    auto tiles_of = [&](int bn) { return w_tiles * ((p.M + bn - 1) / bn); };
+    p.splits = 1;
+    if (p.M > 128) {
+        if (tiles_of(256) <= sms && tiles_of(256) * 4 >= 3ll * sms) return run(256, true, tiles_of(256));
+        if (tiles_of(WIDE) > sms) return run(WIDE, false, tiles_of(WIDE));
+    }
+    const int bn = p.M <= 32 ? 32 : p.M <= 64 ? 64 : 128;
+    const long long tiles = tiles_of(bn);
+    if (tiles > sms) return run(bn, false, tiles);
+    while (p.splits < 8 && tiles * p.splits * 2 <= sms && p.splits * 2 <= chunks) p.splits *= 2;
+    return run(bn, true, tiles);
+}
+
+}  // namespace

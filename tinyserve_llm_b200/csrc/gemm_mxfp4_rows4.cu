@@ -1,0 +1,265 @@
+// Products over microscaled 4-bit weights on tcgen05, rows of x in four bits too.
+//
+// Codes of both sides come by TMA, 256 numbers a row of 128 bytes, and tcgen05.mma kind::mxf4 multiplies them, four times as many a cycle
+// as bfloat16 numbers.  The scales it reads from tensor memory: four warps gather their bytes from global memory, 32 scales of a row at a
+// time (four stages; at one stage's eight bytes the loads of 384 rows, a sector each, took longer than the MMAs), and put a stage's into
+// shared memory, 16 bytes for lane l of which bytes 4 j .. 4 j + 3 belong to row 32 j + l; tcgen05.cp hands them to all four quarters of
+// the lanes.
+#include "gemm_mxfp4.cuh"
+
+namespace {
+
+// Warps: producer, issuer, eight of the epilogue, four that gather scales.
+constexpr int EPI_WARPS = 8, GATHER = 4, THREADS = 32 * (2 + EPI_WARPS + GATHER);
+
+__device__ __forceinline__ void umma(uint32_t leader, uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sa, uint32_t sb,
+                                     uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %6, 0;\n\tsetp.ne.b32 q, %7, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+        ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate), "r"(leader) : "memory");
+}
+// 32 rows of 16 bytes of shared memory into four columns of tensor memory, the same for each quarter of the lanes.
+__device__ __forceinline__ void copy_scales(uint32_t leader, uint32_t tmem, uint64_t desc) {
+    asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %2, 0;\n\t@q tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;\n\t}"
+                 ::"r"(tmem), "l"(desc), "r"(leader) : "memory");
+}
+// Descriptor of 32 rows of 16 bytes that lie one behind the other: groups of eight rows 128 bytes apart, no swizzle.
+__device__ __forceinline__ uint64_t scale_desc(const void* at) {
+    return (uint64_t)((smem_u32(at) & 0x3FFFF) >> 4) | (uint64_t)(128 >> 4) << 32 | (uint64_t)1 << 46;
+}
+// e2m1 x e2m1 -> float32 with scales of power-of-two bytes, two a row and MMA; `pair`: which two of the four bytes of a column.
+__device__ __forceinline__ uint32_t instr_desc(int n, int pair) {
+    return (uint32_t)(2 * pair) << 4 | 1u << 7 | 1u << 10 | (uint32_t)(n >> 3) << 17 | 1u << 23 | (uint32_t)(BM >> 7) << 27 | (uint32_t)(2 * pair) << 29;
+}
+
+template <int BN>
+__host__ __device__ constexpr int x_sets() { return (BN + 127) / 128; }                    // of 128 rows of x's scales
+template <int BN>
+__host__ __device__ constexpr int scale_columns() { return 8 + 8 * x_sets<BN>(); }        // of tensor memory, a stage
+
+template <bool GATED, int BN, int STAGES, bool SPLIT>
+__global__ void __launch_bounds__(THREADS, 1)
+rows4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, MxParams p) {
+    constexpr int B_BYTES = BN * ROW, SCALE_COLS = scale_columns<BN>(), SCALE_BYTES = SCALE_COLS * 128, X_SETS = x_sets<BN>();
+    constexpr int ACCUMULATORS = SPLIT ? 1 : 2, OUTS = GATED ? BM / 2 : BM, SHARE = BN / (EPI_WARPS / 4);
+    constexpr int TMEM_USED = ACCUMULATORS * BN + STAGES * SCALE_COLS, TMEM_COLS = power_of_two(TMEM_USED);
+    static_assert(TMEM_USED <= 512, "tensor memory has 512 columns");
+    static_assert(!SPLIT || BM * BN * 4 <= STAGES * (A_BYTES + B_BYTES), "a split tile's sums go where the ring was");
+    extern __shared__ __align__(1024) unsigned char smem_raw[];
+    __shared__ __align__(8) uint64_t full_bar[STAGES], empty_bar[STAGES], tmem_full_bar[2], tmem_empty_bar[2];
+    __shared__ uint32_t tmem_base_slot;
+    __shared__ int failed;
+
+    unsigned char* stages = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    unsigned char* scale_ring = stages + STAGES * (A_BYTES + B_BYTES);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int outs = GATED ? p.inter : p.N;
+    const int x_tiles = (p.M + BN - 1) / BN, num_tiles = x_tiles * ((outs + OUTS - 1) / OUTS);
+    const int all_chunks = (p.blocks * MX_BLOCK + CHUNK - 1) / CHUNK;
+    const int rank = SPLIT && p.splits > 1 ? (int)pair_rank() : 0;
+    const int first_tile = SPLIT ? (int)blockIdx.x / p.splits : (int)blockIdx.x, tile_step = SPLIT ? num_tiles : (int)gridDim.x;
+    const int chunk0 = SPLIT ? (int)((long long)all_chunks * rank / p.splits) : 0;
+    const int chunk1 = SPLIT ? (int)((long long)all_chunks * (rank + 1) / p.splits) : all_chunks;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < STAGES; ++s) {
+            mbar_init(&full_bar[s], 1 + GATHER);     // the producer's bytes, and the warps that write shared memory
+            mbar_init(&empty_bar[s], 1);
+        }
+        for (int b = 0; b < 2; ++b) {
+            mbar_init(&tmem_full_bar[b], 1);
+            mbar_init(&tmem_empty_bar[b], EPI_WARPS);
+        }
+        failed = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base_slot)), "r"(TMEM_COLS) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const uint32_t tmem_base = tmem_base_slot;
+
+    chain_wait();                                    // x, or the weights themselves, may come from a kernel ahead on the stream
+    chain_release();
+
+    if (warp == 0) {
+        // ---------------------------------------------------------------- TMA producer
+        if (lane == 0) {
+            Ring<STAGES> r;
+            for (int tile = first_tile; tile < num_tiles && !failed; tile += tile_step) {
+                const int t0 = (tile % x_tiles) * BN, f0 = (tile / x_tiles) * OUTS;
+                for (int chunk = chunk0; chunk < chunk1; ++chunk, r.next()) {
+                    const int s = r.at;
+                    if (!wait_for(&empty_bar[s], r.parity ^ 1, p.error, 41)) { failed = 1; break; }
+                    unsigned char* tile_at = stages + s * (A_BYTES + B_BYTES);
+                    mbar_expect_tx(&full_bar[s], A_BYTES + B_BYTES);
+                    load_codes<GATED>(tile_at, &map_w, &full_bar[s], p, chunk, f0);
+                    tma_load_2d(tile_at + A_BYTES, &map_x, &full_bar[s], chunk * ROW, t0);
+                }
+            }
+        }
+    } else if (warp == 1) {
+        // ---------------------------------------------------------------- MMA issuer
+        const uint32_t leader = elect_one();
+        const uint32_t tmem_scales = tmem_base + ACCUMULATORS * BN;
+        bool ok = true;                              // the same in all lanes
+        Ring<STAGES> r;
+        const uint64_t a_first = smem_desc(stages), b_first = smem_desc(stages + A_BYTES), scales_first = scale_desc(scale_ring);
+        int iter = 0;
+        for (int tile = first_tile; tile < num_tiles && ok; tile += tile_step, ++iter) {
+            const int buf = SPLIT ? 0 : iter & 1;
+            ok = __all_sync(0xffffffffu, mbar_wait(&tmem_empty_bar[buf], ((iter >> 1) & 1) ^ 1, p.error, 44) && !failed);
+            if (!ok) { failed = 1; break; }
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            const uint32_t tmem_d = tmem_base + buf * BN;
+            uint32_t add = 0;                        // the tile's first MMA starts its sums
+            for (int left = chunk1 - chunk0; left > 0; --left, r.next()) {
+                ok = __all_sync(0xffffffffu, wait_for(&full_bar[r.at], r.parity, p.error, 42));
+                if (!ok) { failed = 1; break; }
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                const uint64_t a_desc = a_first + r.at * ((A_BYTES + B_BYTES) / 16), b_desc = b_first + r.at * ((A_BYTES + B_BYTES) / 16);
+                const uint64_t from = scales_first + r.at * (SCALE_BYTES / 16);
+                // a stage's scales have columns of their own: they are free when the stage is, once the MMAs that read them have retired
+                const uint32_t sa = tmem_scales + r.at * SCALE_COLS, sb = sa + 8;
+#pragma unroll
+                for (int i = 0; i < 2 + 2 * X_SETS; ++i) copy_scales(leader, sa + 4 * i, from + 32 * i);
+#pragma unroll
+                for (int k = 0; k < 4; ++k, add = 1)  // 64 columns of K are 32 bytes and two scales a row
+                    umma(leader, tmem_d, a_desc + 2 * k, b_desc + 2 * k, instr_desc(BN, k & 1), sa + (k >> 1) * 4, sb + (k >> 1) * 4 * X_SETS, add);
+                if (leader) umma_commit(&empty_bar[r.at]);
+            }
+            if (leader) umma_commit(&tmem_full_bar[buf]);
+        }
+    } else if (warp < 2 + EPI_WARPS) {
+        // ---------------------------------------------------------------- epilogue
+        const int quarter = warp & 3, first = ((warp - 2) >> 2) * SHARE;      // the 32 lanes this warp may read; its share of the columns
+        const bool paired = ((outs | (int)(p.ldy & 1)) & 1) == 0 && ((uintptr_t)p.y & 3) == 0;
+        int iter = 0;
+        for (int tile = first_tile; tile < num_tiles; tile += tile_step, ++iter) {
+            const int buf = SPLIT ? 0 : iter & 1;
+            const int t0 = (tile % x_tiles) * BN, f0 = (tile / x_tiles) * OUTS;
+            const bool ok = mbar_wait(&tmem_full_bar[buf], (iter >> 1) & 1, p.error, 43) && !failed;
+            if (!__all_sync(0xffffffffu, ok)) { failed = 1; break; }
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            finish_tile<GATED, SHARE, SPLIT>(p, tmem_base + buf * BN, first, t0, f0, outs, paired, quarter, lane, reinterpret_cast<float*>(stages),
+                                             &tmem_empty_bar[buf]);
+        }
+    } else {
+        // ---------------------------------------------------------------- scales
+        // Groups of 32 rows, a row a lane: 0 to 3 of W, from 4 on of x; a warp has every fourth.  What a group leaves out of its 512 bytes
+        // (fewer than 128 rows of x) belongs to columns that no MMA reads.
+        constexpr int GROUPS = 4 + BN / 32, MINE = (GROUPS + GATHER - 1) / GATHER;
+        const int w = warp - 2 - EPI_WARPS;
+        bool ok = true;
+        Ring<STAGES> r;
+        for (int tile = first_tile; tile < num_tiles && ok; tile += tile_step) {
+            const int t0 = (tile % x_tiles) * BN, f0 = (tile / x_tiles) * OUTS;
+            const uint8_t* row[MINE];
+#pragma unroll
+            for (int i = 0; i < MINE; ++i) {
+                const int g = w + i * GATHER;
+                row[i] = g < 4 ? p.w_scales + (long long)min(row_of<GATED>(p, f0, g * 32 + lane), p.N - 1) * p.w_ld_scales
+                               : p.x_scales + (long long)min(t0 + (g - 4) * 32 + lane, p.M - 1) * p.x_ld_scales;
+            }
+            auto load = [&](int four, uint4 (&v)[MINE][2]) {          // 32 scales of each row, four chunks' worth; behind the last block 1
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int b = four * 32 + h * 16;
+#pragma unroll
+                    for (int i = 0; i < MINE; ++i) {
+                        if (w + i * GATHER >= GROUPS) continue;
+                        if (b + 16 <= p.blocks) {
+                            v[i][h] = __ldg(reinterpret_cast<const uint4*>(row[i] + b));
+                        } else if (b < p.blocks) {
+                            uint32_t q[4] = {0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu};
+#pragma unroll
+                            for (int j = 0; j < 16; ++j)
+                                if (b + j < p.blocks) q[j >> 2] = (q[j >> 2] & ~(0xffu << (8 * (j & 3)))) | (uint32_t)row[i][b + j] << (8 * (j & 3));
+                            v[i][h] = make_uint4(q[0], q[1], q[2], q[3]);
+                        }
+                    }
+                }
+            };
+            uint4 now[MINE][2], next[MINE][2];
+            load(chunk0 >> 2, now);
+            for (int chunk = chunk0; chunk < chunk1; ++chunk, r.next()) {
+                const int s = r.at;
+                if (((chunk & 3) == 0 || chunk == chunk0) && (chunk | 3) + 1 < chunk1) load((chunk >> 2) + 1, next);
+                ok = __all_sync(0xffffffffu, wait_for(&empty_bar[s], r.parity ^ 1, p.error, 45) && !failed);
+                if (!ok) { failed = 1; break; }
+#pragma unroll
+                for (int i = 0; i < MINE; ++i) {
+                    const int g = w + i * GATHER;
+                    if (g >= GROUPS) continue;
+                    const uint4 v = chunk & 2 ? now[i][1] : now[i][0];
+                    unsigned char* to = scale_ring + s * SCALE_BYTES + lane * 16 + (g & 3) * 4 + (g < 4 ? 0 : 1024 + ((g - 4) >> 2) * 512);
+                    *reinterpret_cast<uint32_t*>(to) = chunk & 1 ? v.z : v.x;
+                    *reinterpret_cast<uint32_t*>(to + (g < 4 ? 512 : X_SETS * 512)) = chunk & 1 ? v.w : v.y;
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&full_bar[s]);
+                if ((chunk & 3) == 3) {
+#pragma unroll
+                    for (int i = 0; i < MINE; ++i) now[i][0] = next[i][0], now[i][1] = next[i][1];
+                }
+            }
+        }
+    }
+    __syncwarp();
+    if (SPLIT && p.splits > 1) {
+        pair_sync();                                 // every CTA's sums are in its shared memory
+        if (warp >= 2 && warp < 2 + EPI_WARPS) {
+            const int t0 = (first_tile % x_tiles) * BN, f0 = (first_tile / x_tiles) * OUTS;
+            join_splits<GATED>(p, smem_u32(stages), rank, min(BN, p.M - t0), t0, f0, outs, threadIdx.x - 64, 32 * EPI_WARPS);
+        }
+        __syncwarp();
+        pair_sync();                                 // nobody reads another CTA's sums any more
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    if (failed) {                                    // copies and MMAs still under way get some half a millisecond before the CTA goes
+        const long long start = clock64();
+        while (clock64() - start < 1000000) {}
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(TMEM_COLS) : "memory");
+    }
+}
+
+template <bool GATED, int BN, int STAGES, bool SPLIT>
+int run(const void* x, long long ldx, MxParams& p, long long tiles, int sms, int device, cudaStream_t stream) {
+    CUtensorMap map_w, map_x;
+    if (make_codes_map<GATED>(&map_w, p)) return 1;
+    if (make_tile_map(&map_x, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, x, p.M, (long long)p.blocks * 16, ldx, BN, "gemm_mxfp4")) return 1;
+    static unsigned long long allowed = 0;
+    return launch_mxfp4(rows4_kernel<GATED, BN, STAGES, SPLIT>, allowed, THREADS,
+                        (size_t)STAGES * (A_BYTES + BN * ROW + 128 * scale_columns<BN>()) + 1024, SPLIT, tiles, sms, device, map_w, map_x, p, stream);
+}
+
+template <bool GATED>
+int dispatch(const void* x, long long ldx, MxParams& p, cudaStream_t stream) {
+    int sms = 148, device = 0;
+    if (cudaGetDevice(&device) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
+    return cut_mxfp4<GATED, 192>(p, sms, [&](int bn, bool split, long long tiles) {
+        if (bn == 256) return run<GATED, 256, 4, true>(x, ldx, p, tiles, sms, device, stream);
+        if (bn == 192) return run<GATED, 192, 5, false>(x, ldx, p, tiles, sms, device, stream);
+        if (bn == 128) return split ? run<GATED, 128, 6, true>(x, ldx, p, tiles, sms, device, stream)
+                                    : run<GATED, 128, 6, false>(x, ldx, p, tiles, sms, device, stream);
+        if (bn == 64) return split ? run<GATED, 64, 8, true>(x, ldx, p, tiles, sms, device, stream)
+                                   : run<GATED, 64, 8, false>(x, ldx, p, tiles, sms, device, stream);
+        return split ? run<GATED, 32, 8, true>(x, ldx, p, tiles, sms, device, stream)
+                     : run<GATED, 32, 8, false>(x, ldx, p, tiles, sms, device, stream);
+    });
+}
+
+}  // namespace
+
+int mxfp4_rows4(const void* x, long long ldx, MxParams& p, int gated, cudaStream_t stream) {
+    return gated ? dispatch<true>(x, ldx, p, stream) : dispatch<false>(x, ldx, p, stream);
+}

@@ -110,7 +110,7 @@ _SIGNATURES = {
     "ts_scale_tanh_cap": ("int", "plffp"),
     "ts_quantize_mxfp4": ("int", "ppplilllip"),
     "ts_dequantize_mxfp4": ("int", "ppplillip"),
-    "ts_gemm_mxfp4": ("int", "ppllplplp" "iiil" "iiffipp"),
+    "ts_gemm_mxfp4": ("int", "ppllplplp" "iiil" "iiffiipp"),
 }
 _CTYPES = {"p": ctypes.c_void_p, "i": ctypes.c_int, "l": ctypes.c_longlong, "f": ctypes.c_float}
 _RETURNS = {"int": ctypes.c_int, "long long": ctypes.c_longlong, "void": None, "const char*": ctypes.c_char_p}
@@ -146,7 +146,9 @@ _WAIT_CODES: dict[int, tuple[str, str]] = {
     43: ("gemm_mxfp4", "epilogue waiting for an accumulator"),
     44: ("gemm_mxfp4", "MMA issuer waiting for a drained accumulator"),
     45: ("gemm_mxfp4", "warps of the scales waiting for a free ring slot"),
-    46: ("gemm_mxfp4", "warps that spread codes waiting for a free ring slot"),
+    46: ("gemm_mxfp4", "warps that spread codes waiting for free tensor memory"),
+    47: ("gemm_mxfp4", "TMA producer of codes waiting for a free buffer"),
+    48: ("gemm_mxfp4", "warps that spread codes waiting for a chunk of them"),
 }
 
 
@@ -1667,12 +1669,13 @@ class Ops:
 
     # ------------------------------------------------------------------ microscaled 4-bit floating point
     @staticmethod
-    def _check_here(device: torch.device, name: str) -> None:
+    def _check_here(t: torch.Tensor, name: str) -> None:
         """The kernels run on the current device's current stream: what they read has to lie there."""
-        if device.type != "cuda":
+        if not t.is_cuda:
             raise KernelError(f"{name} must be on a CUDA device; the engine has no CPU path")
-        if device.index is not None and device.index != torch.cuda.current_device():
-            raise KernelError(f"{name} is on {device}, the current device is cuda:{torch.cuda.current_device()}")
+        here = _RAW_DEVICE() if _RAW_DEVICE is not None else torch.cuda.current_device()
+        if t.get_device() != here:
+            raise KernelError(f"{name} is on {t.device}, the current device is cuda:{here}")
 
     def quantize_mxfp4(self, x: torch.Tensor) -> MXFP4:
         """
@@ -1685,7 +1688,7 @@ class Ops:
         rows, cols = x.shape
         if cols == 0:
             raise KernelError("quantize_mxfp4: x has no columns")
-        self._check_here(x.device, "x")
+        self._check_here(x, "x")
         q = MXFP4.empty(rows, cols, x.device)
         if rows:
             self._call("ts_quantize_mxfp4", _ptr(x), _ptr(q.codes), _ptr(q.scales), rows, cols, x.stride(0) if rows > 1 else cols, q.ld_codes,
@@ -1696,7 +1699,7 @@ class Ops:
         """The numbers q stands for, [rows, cols] in bfloat16 or float32: exact, but for what the type has no room for (infinite)."""
         if dtype not in _DTYPE_CODE:
             raise KernelError(f"dequantize_mxfp4: dtype {dtype}, expected one of {tuple(_DTYPE_CODE)}")
-        self._check_here(q.device, "q")
+        self._check_here(q.codes, "q")
         out = torch.empty((q.rows, q.cols), dtype=dtype, device=q.device)
         if q.rows:
             self._call("ts_dequantize_mxfp4", _ptr(q.codes), _ptr(q.scales), _ptr(out), q.rows, q.cols, q.ld_codes, q.ld_scales,
@@ -1728,33 +1731,40 @@ class Ops:
 
     def _product_mxfp4(self, who: str, x: torch.Tensor | MXFP4, w: MXFP4, activation: str | None, limit: float, alpha: float,
                        out_dtype: torch.dtype, out: torch.Tensor | None) -> torch.Tensor:
+        M, K, N = -1, -1, w.rows
         both = isinstance(x, MXFP4)
-        M, K = (x.rows, x.cols) if both else tuple(x.shape) if x.dim() == 2 else (-1, -1)
-        if M < 0 or K != w.cols:
-            raise KernelError(f"{who}: x is {tuple(x.codes.shape if both else x.shape)}, the weight has rows of {w.cols} numbers")
-        self._check_here(w.device, "weight")
-        self._check_here(x.device, "x")
-        if not both:
-            if x.dtype != torch.bfloat16:
-                raise KernelError(f"{who}: x has dtype {x.dtype}; the products over 4-bit weights take bfloat16 or quantised rows")
-            ldx = x.stride(0) if M > 1 else K
-            if K % 8 or (K > 1 and x.stride(1) != 1) or ldx % 8 or ldx < K or x.data_ptr() % 16:
-                raise KernelError(f"{who}: x must have a multiple of 8 columns, contiguous, in rows that start 16-byte aligned "
-                                  f"(shape {tuple(x.shape)}, strides {x.stride()})")
-        cols = w.rows if activation is None else w.rows // 2
+        if both:
+            M, K, rows, ldx, x_scales, x_ld_scales = x.rows, x.cols, x.codes, x.ld_codes, x.scales.data_ptr(), x.ld_scales
+        else:
+            rows, ldx, x_scales, x_ld_scales = x, 0, 0, 0
+            if x.dim() == 2:
+                M, K = x.shape
+                ldx, one = x.stride()
+                if M <= 1:
+                    ldx = K
+                if x.dtype is not torch.bfloat16:
+                    raise KernelError(f"{who}: x has dtype {x.dtype}; the products over 4-bit weights take bfloat16 or quantised rows")
+                if K % 8 or one != 1 or ldx % 8 or ldx < K or x.data_ptr() % 16:
+                    raise KernelError(f"{who}: x must have a multiple of 8 columns, contiguous, in rows that start 16-byte aligned "
+                                      f"(shape {tuple(x.shape)}, strides {x.stride()})")
+        if K != w.cols:
+            raise KernelError(f"{who}: x is {tuple(rows.shape) if not both else (M, K)}, the weight has rows of {w.cols} numbers")
+        self._check_here(w.codes, "weight")
+        self._check_here(rows, "x")
+        cols = N if activation is None else N // 2
         if out is None:
-            out = torch.empty((M, cols), dtype=out_dtype, device=w.device)
+            out = torch.empty((M, cols), dtype=out_dtype, device=rows.device)
         else:
             self._check(out, "out", out_dtype, 2)
-            self._check_here(out.device, "out")
+            self._check_here(out, "out")
             if tuple(out.shape) != (M, cols):
                 raise KernelError(f"{who}: out is {tuple(out.shape)}, the product {(M, cols)}")
         if M == 0 or cols == 0:
             return out
         kind = 0 if activation is None else self.GATED_ACTIVATIONS[activation]
-        self._call("ts_gemm_mxfp4", _ptr(w.codes), _ptr(w.scales), w.ld_codes, w.ld_scales, _ptr(x.codes) if both else _ptr(x),
-                   x.ld_codes if both else ldx, _ptr(x.scales) if both else 0, x.ld_scales if both else 0, _ptr(out), M, w.rows, K, cols,
-                   0 if activation is None else 1, kind, limit, alpha, _DTYPE_CODE[out_dtype], self.error_word().data_ptr(), _stream())
+        self._call("ts_gemm_mxfp4", w.codes.data_ptr(), w.scales.data_ptr(), w.ld_codes, w.ld_scales, rows.data_ptr(), ldx, x_scales, x_ld_scales,
+                   out.data_ptr(), M, N, K, cols, 0 if activation is None else 1, kind, limit, alpha, 1 if w.settled else 0,
+                   _DTYPE_CODE[out_dtype], self.error_word().data_ptr(), _stream())
         return out
 
     def linear_columns(self, x: torch.Tensor, weight: torch.Tensor, out_dtype: torch.dtype | None = None) -> torch.Tensor:
