@@ -31,6 +31,8 @@ struct MxParams {
     int out_f32, act;
     float act_limit, act_alpha;
     int one_box;                                       // gated: a tile's codes are one box of a map of four dimensions
+    const __nv_bfloat16* x16;                          // rows in bfloat16 that came in pieces: themselves
+    long long x16_ld;
     int settled;                                       // W may be read before the kernels ahead on the stream have finished
     int splits;
     int* error;
@@ -39,6 +41,9 @@ struct MxParams {
 // Either form's products: the launcher's checks have been made.
 int mxfp4_rows16(const void* x, long long ldx, MxParams& p, int gated, cudaStream_t stream);
 int mxfp4_rows4(const void* x, long long ldx, MxParams& p, int gated, cudaStream_t stream);
+// A few rows in bfloat16 as pieces of four bits, which take `scratch`.
+long long mxfp4_pieces_bytes(int M, int blocks);
+int mxfp4_pieces(const void* x, long long ldx, void* scratch, MxParams& p, int gated, cudaStream_t stream);
 
 namespace {
 
@@ -216,32 +221,60 @@ __device__ __forceinline__ void finish_tile(const MxParams& p, uint32_t tmem, in
     }
 }
 
-// A split tile's share of columns, added up over the cluster's CTAs by `threads` threads, `id` of them this one.
-template <bool GATED>
-__device__ __forceinline__ void join_splits(const MxParams& p, uint32_t sums, int rank, int columns, int t0, int f0, int outs, int id, int threads) {
-    constexpr int OUTS = GATED ? BM / 2 : BM;
-    auto total = [&](int column, int l) {
-        float v = 0.f;
-        for (int r = 0; r < p.splits; ++r) {
-            uint32_t remote;
-            float part;
-            asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(sums + (uint32_t)(column * BM + l) * 4), "r"(r));
-            asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(part) : "r"(remote));
-            v += part;
+// A split tile's share of columns, added up over the cluster's CTAs, four neighbouring lanes a thread: `id` of `threads` this one.
+// `again` works out what comes out as NaN, where that may be more than a NaN among the factors.
+template <bool GATED, typename Again>
+__device__ __forceinline__ void join_splits(const MxParams& p, uint32_t sums, int rank, int columns, int t0, int f0, int outs, int id, int threads,
+                                            const Again& again) {
+    constexpr int QUADS = (GATED ? BM / 2 : BM) / 4;
+    auto total = [&](int column, int l, float (&v)[4]) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = 0.f;
+        for (int r0 = 0; r0 < p.splits; r0 += 4) {                    // four asked for before the first is added
+            float part[4][4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                if (r0 + r >= p.splits) break;
+                uint32_t remote;
+                asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(sums + (uint32_t)(column * BM + l) * 4), "r"(r0 + r));
+                asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                             : "=f"(part[r][0]), "=f"(part[r][1]), "=f"(part[r][2]), "=f"(part[r][3]) : "r"(remote));
+            }
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                if (r0 + r >= p.splits) break;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] += part[r][e];
+            }
         }
-        return v;
     };
-    const int f = id % OUTS;
-    if (f0 + f >= outs) return;
-    for (int c = rank + p.splits * (id / OUTS); c < columns; c += p.splits * (threads / OUTS)) {
+    const int f = (id % QUADS) * 4;
+    for (int c = rank + p.splits * (id / QUADS); c < columns && id / QUADS < threads / QUADS; c += p.splits * (threads / QUADS)) {
         const long long at = (long long)(t0 + c) * p.ldy + f0 + f;
+        float v[4];
         if (GATED) {
             const int l = (f >> 4) * 32 + (f & 15);
-            ((__nv_bfloat16*)p.y)[at] = __float2bfloat16_rn(gate_one(p, total(c, l), total(c, l + 16)));
-        } else if (p.out_f32) {
-            ((float*)p.y)[at] = total(c, f);
+            float u[4];
+            total(c, l, v);
+            total(c, l + 16, u);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                if (f0 + f + e >= outs) break;
+                if (v[e] != v[e]) v[e] = again(l + e, t0 + c);
+                if (u[e] != u[e]) u[e] = again(l + 16 + e, t0 + c);
+                v[e] = gate_one(p, v[e], u[e]);
+            }
         } else {
-            ((__nv_bfloat16*)p.y)[at] = __float2bfloat16_rn(total(c, f));
+            total(c, f, v);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (f0 + f + e < outs && v[e] != v[e]) v[e] = again(f + e, t0 + c);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            if (f0 + f + e >= outs) break;
+            if (!GATED && p.out_f32) ((float*)p.y)[at + e] = v[e];
+            else ((__nv_bfloat16*)p.y)[at + e] = __float2bfloat16_rn(v[e]);
         }
     }
 }
@@ -279,21 +312,28 @@ int launch_mxfp4(Kernel kernel, unsigned long long& allowed, int threads, size_t
     return 0;
 }
 
-// How a product is cut.  run(bn, split) launches tiles of bn rows of x (WIDE, 256, 128, 64, 32).
-template <bool GATED, int WIDE, typename Run>
-int cut_mxfp4(MxParams& p, int sms, const Run& run) {
-    const long long outs = GATED ? p.inter : p.N, per = GATED ? BM / 2 : BM, w_tiles = (outs + per - 1) / per;
+// CTAs a tile: as many as there are SMs for, up to a cluster's eight and the chunks of K.
+inline int splits_of(const MxParams& p, long long tiles, int sms) {
     const int chunks = (p.blocks * MX_BLOCK + CHUNK - 1) / CHUNK;
-    auto tiles_of = [&](int bn) { return w_tiles * ((p.M + bn - 1) / bn); };
+    int splits = 1;
+    while (splits < 8 && tiles * splits * 2 <= sms && splits * 2 <= chunks) splits *= 2;
+    return splits;
+}
+
+// How a product is cut.  run(bn, split, tiles) launches tiles of bn rows of x (WIDE, 256, 128, 64, 32).
+template <bool GATED, int WIDE, typename Run>
+int cut_mxfp4(MxParams& p, int rows, int sms, const Run& run) {
+    const long long outs = GATED ? p.inter : p.N, per = GATED ? BM / 2 : BM, w_tiles = (outs + per - 1) / per;
+    auto tiles_of = [&](int bn) { return w_tiles * ((rows + bn - 1) / bn); };
     p.splits = 1;
-    if (p.M > 128) {
+    if (rows > 128) {
         if (tiles_of(256) <= sms && tiles_of(256) * 4 >= 3ll * sms) return run(256, true, tiles_of(256));
         if (tiles_of(WIDE) > sms) return run(WIDE, false, tiles_of(WIDE));
     }
-    const int bn = p.M <= 32 ? 32 : p.M <= 64 ? 64 : 128;
+    const int bn = rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
     const long long tiles = tiles_of(bn);
     if (tiles > sms) return run(bn, false, tiles);
-    while (p.splits < 8 && tiles * p.splits * 2 <= sms && p.splits * 2 <= chunks) p.splits *= 2;
+    p.splits = splits_of(p, tiles, sms);
     return run(bn, true, tiles);
 }
 

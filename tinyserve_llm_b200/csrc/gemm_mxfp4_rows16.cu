@@ -235,10 +235,9 @@ rows16_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
     __syncwarp();
     if (SPLIT && p.splits > 1) {
         pair_sync();                                 // every CTA's sums are in its shared memory
-        if (warp >= 2 && warp < 2 + EPI_WARPS) {
-            const int t0 = (first_tile % x_tiles) * BN, f0 = (first_tile / x_tiles) * OUTS;
-            join_splits<GATED>(p, smem_u32(stages), rank, min(BN, p.M - t0), t0, f0, outs, threadIdx.x - 64, 32 * EPI_WARPS);
-        }
+        const int t0 = (first_tile % x_tiles) * BN, f0 = (first_tile / x_tiles) * OUTS;
+        join_splits<GATED>(p, smem_u32(stages), rank, min(BN, p.M - t0), t0, f0, outs, threadIdx.x, THREADS,
+                           [](int, int) { return __int_as_float(0x7fffffff); });
         __syncwarp();
         pair_sync();                                 // nobody reads another CTA's sums any more
     }
@@ -268,7 +267,7 @@ template <bool GATED>
 int dispatch(const void* x, long long ldx, MxParams& p, cudaStream_t stream) {
     int sms = 148, device = 0;
     if (cudaGetDevice(&device) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
-    return cut_mxfp4<GATED, 192>(p, sms, [&](int bn, bool split, long long tiles) {
+    return cut_mxfp4<GATED, 192>(p, p.M, sms, [&](int bn, bool split, long long tiles) {
         if (bn == 256) return run<GATED, 256, 5, 3, true>(x, ldx, p, tiles, sms, device, stream);
         if (bn == 192) return run<GATED, 192, 6, 4, false>(x, ldx, p, tiles, sms, device, stream);
         if (bn == 128) return split ? run<GATED, 128, 8, 4, true>(x, ldx, p, tiles, sms, device, stream)

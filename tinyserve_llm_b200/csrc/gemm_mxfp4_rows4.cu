@@ -5,6 +5,12 @@
 // time (four stages; at one stage's eight bytes the loads of 384 rows, a sector each, took longer than the MMAs), and put a stage's into
 // shared memory, 16 bytes for lane l of which bytes 4 j .. 4 j + 3 belong to row 32 j + l; tcgen05.cp hands them to all four quarters of
 // the lanes.
+//
+// A few rows of bfloat16 numbers take the same way (PIECES = 8): each row becomes eight rows of four-bit numbers, what the ones before left
+// quantised again, whose products are added up.  A piece leaves at most a quarter of a block's largest magnitude, so what is lost lies below
+// 2^-16 of it, and every bit of a number that is not 2^9 times smaller than its block's largest is kept.  An MMA of 64 columns costs next to
+// nothing beside the stream of W, where spreading W's codes to bfloat16, here or in registers, takes longer than bringing them (28,672 rows
+// of 4,096, eight rows of x: 41 us).  Infinities have no place in four bits: a result that comes out as NaN is worked out again, number by number.
 #include "gemm_mxfp4.cuh"
 
 namespace {
@@ -38,14 +44,77 @@ __host__ __device__ constexpr int x_sets() { return (BN + 127) / 128; }         
 template <int BN>
 __host__ __device__ constexpr int scale_columns() { return 8 + 8 * x_sets<BN>(); }        // of tensor memory, a stage
 
-template <bool GATED, int BN, int STAGES, bool SPLIT>
-__global__ void __launch_bounds__(THREADS, 1)
+constexpr int PIECES8 = 8;
+
+// One product of a row of W with a bfloat16 row of x, number by number.
+__device__ __noinline__ float plain_dot(const uint8_t* codes, const uint8_t* scales, const __nv_bfloat16* x, int K) {
+    float sum = 0.f;
+    for (int i = 0; i < K; ++i) {
+        const uint32_t byte = codes[i >> 1];
+        sum = fmaf(mx_code_value(i & 1 ? byte >> 4 : byte & 15) * mx_scale(scales[i / MX_BLOCK]), to_float(x[i]), sum);
+    }
+    return sum;
+}
+__device__ __forceinline__ float plain_dot(const MxParams& p, int row, int t) {
+    return plain_dot(p.w_codes + row * p.w_ld_codes, p.w_scales + row * p.w_ld_scales, p.x16 + t * p.x16_ld, p.K);
+}
+
+// The columns of a tile whose x came in pieces, eight a row: an epilogue warp's share, 16 columns, two rows of x, at a time.
+template <bool GATED, int SHARE>
+__device__ __forceinline__ void finish_pieces(const MxParams& p, uint32_t tmem, int first, int t0, int f0, int outs, int quarter, int lane, float* sums) {
+    const uint32_t addr = tmem + first + ((uint32_t)(quarter * 32) << 16);
+    const int f = GATED ? f0 + quarter * 16 + (lane & 15) : f0 + quarter * 32 + lane;
+#pragma unroll 1
+    for (int c0 = 0; c0 < SHARE; c0 += 16) {
+        uint32_t acc[16];
+        __syncwarp();
+        tmem_ld16(addr + c0, acc);
+        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+        const int column = (first + c0) / PIECES8, t = t0 + column;
+        float v[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            v[j] = __uint_as_float(acc[8 * j + 7]);                   // the smallest first
+#pragma unroll
+            for (int i = 6; i >= 0; --i) v[j] += __uint_as_float(acc[8 * j + i]);
+        }
+        if (p.splits > 1) {
+#pragma unroll
+            for (int j = 0; j < 2; ++j) sums[(column + j) * BM + quarter * 32 + lane] = v[j];
+            continue;
+        }
+        if (t >= p.M) continue;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const int row = row_of<GATED>(p, f0, quarter * 32 + lane);
+            if (v[j] != v[j] && t + j < p.M && row < p.N) v[j] = plain_dot(p, row, t + j);
+        }
+        __syncwarp();
+        if (GATED) {                                                  // the lower half of the lanes finishes the first row, the upper one the second
+            const float other = __shfl_xor_sync(0xffffffffu, lane < 16 ? v[1] : v[0], 16);
+            const float y = lane < 16 ? gate_one(p, v[0], other) : gate_one(p, other, v[1]);
+            if (t + (lane >> 4) < p.M && f < outs) ((__nv_bfloat16*)p.y)[(long long)(t + (lane >> 4)) * p.ldy + f] = __float2bfloat16_rn(y);
+        } else if (f < outs) {
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                if (t + j >= p.M) break;
+                if (p.out_f32) ((float*)p.y)[(long long)(t + j) * p.ldy + f] = v[j];
+                else ((__nv_bfloat16*)p.y)[(long long)(t + j) * p.ldy + f] = __float2bfloat16_rn(v[j]);
+            }
+        }
+    }
+}
+
+// Tiles of up to 64 columns leave room for two CTAs an SM, so that one's beginning and end run beside the other's stream of W.
+template <bool GATED, int BN, int STAGES, bool SPLIT, int PIECES>
+__global__ void __launch_bounds__(THREADS, BN <= 64 ? 2 : 1)
 rows4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, MxParams p) {
     constexpr int B_BYTES = BN * ROW, SCALE_COLS = scale_columns<BN>(), SCALE_BYTES = SCALE_COLS * 128, X_SETS = x_sets<BN>();
     constexpr int ACCUMULATORS = SPLIT ? 1 : 2, OUTS = GATED ? BM / 2 : BM, SHARE = BN / (EPI_WARPS / 4);
     constexpr int TMEM_USED = ACCUMULATORS * BN + STAGES * SCALE_COLS, TMEM_COLS = power_of_two(TMEM_USED);
     static_assert(TMEM_USED <= 512, "tensor memory has 512 columns");
-    static_assert(!SPLIT || BM * BN * 4 <= STAGES * (A_BYTES + B_BYTES), "a split tile's sums go where the ring was");
+    static_assert(PIECES == 1 || SPLIT, "pieces are added up by tiles");
+    static_assert(!SPLIT || BM * BN / PIECES * 4 <= STAGES * (A_BYTES + B_BYTES), "a split tile's sums go where the ring was");
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     __shared__ __align__(8) uint64_t full_bar[STAGES], empty_bar[STAGES], tmem_full_bar[2], tmem_empty_bar[2];
     __shared__ uint32_t tmem_base_slot;
@@ -55,7 +124,7 @@ rows4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
     unsigned char* scale_ring = stages + STAGES * (A_BYTES + B_BYTES);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int outs = GATED ? p.inter : p.N;
-    const int x_tiles = (p.M + BN - 1) / BN, num_tiles = x_tiles * ((outs + OUTS - 1) / OUTS);
+    const int x_tiles = (p.M * PIECES + BN - 1) / BN, num_tiles = x_tiles * ((outs + OUTS - 1) / OUTS);
     const int all_chunks = (p.blocks * MX_BLOCK + CHUNK - 1) / CHUNK;
     const int rank = SPLIT && p.splits > 1 ? (int)pair_rank() : 0;
     const int first_tile = SPLIT ? (int)blockIdx.x / p.splits : (int)blockIdx.x, tile_step = SPLIT ? num_tiles : (int)gridDim.x;
@@ -91,14 +160,14 @@ rows4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
         if (lane == 0) {
             Ring<STAGES> r;
             for (int tile = first_tile; tile < num_tiles && !failed; tile += tile_step) {
-                const int t0 = (tile % x_tiles) * BN, f0 = (tile / x_tiles) * OUTS;
+                const int t0 = (tile % x_tiles) * (BN / PIECES), f0 = (tile / x_tiles) * OUTS;
                 for (int chunk = chunk0; chunk < chunk1; ++chunk, r.next()) {
                     const int s = r.at;
                     if (!wait_for(&empty_bar[s], r.parity ^ 1, p.error, 41)) { failed = 1; break; }
                     unsigned char* tile_at = stages + s * (A_BYTES + B_BYTES);
                     mbar_expect_tx(&full_bar[s], A_BYTES + B_BYTES);
                     load_codes<GATED>(tile_at, &map_w, &full_bar[s], p, chunk, f0);
-                    tma_load_2d(tile_at + A_BYTES, &map_x, &full_bar[s], chunk * ROW, t0);
+                    tma_load_2d(tile_at + A_BYTES, &map_x, &full_bar[s], chunk * ROW, t0 * PIECES);
                 }
             }
         }
@@ -141,12 +210,15 @@ rows4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
         int iter = 0;
         for (int tile = first_tile; tile < num_tiles; tile += tile_step, ++iter) {
             const int buf = SPLIT ? 0 : iter & 1;
-            const int t0 = (tile % x_tiles) * BN, f0 = (tile / x_tiles) * OUTS;
+            const int t0 = (tile % x_tiles) * (BN / PIECES), f0 = (tile / x_tiles) * OUTS;
             const bool ok = mbar_wait(&tmem_full_bar[buf], (iter >> 1) & 1, p.error, 43) && !failed;
             if (!__all_sync(0xffffffffu, ok)) { failed = 1; break; }
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            finish_tile<GATED, SHARE, SPLIT>(p, tmem_base + buf * BN, first, t0, f0, outs, paired, quarter, lane, reinterpret_cast<float*>(stages),
-                                             &tmem_empty_bar[buf]);
+            if (PIECES > 1)
+                finish_pieces<GATED, SHARE>(p, tmem_base, first, t0, f0, outs, quarter, lane, reinterpret_cast<float*>(stages));
+            else
+                finish_tile<GATED, SHARE, SPLIT>(p, tmem_base + buf * BN, first, t0, f0, outs, paired, quarter, lane, reinterpret_cast<float*>(stages),
+                                                 &tmem_empty_bar[buf]);
         }
     } else {
         // ---------------------------------------------------------------- scales
@@ -157,13 +229,13 @@ rows4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
         bool ok = true;
         Ring<STAGES> r;
         for (int tile = first_tile; tile < num_tiles && ok; tile += tile_step) {
-            const int t0 = (tile % x_tiles) * BN, f0 = (tile / x_tiles) * OUTS;
+            const int t0 = (tile % x_tiles) * (BN / PIECES), f0 = (tile / x_tiles) * OUTS;
             const uint8_t* row[MINE];
 #pragma unroll
             for (int i = 0; i < MINE; ++i) {
                 const int g = w + i * GATHER;
                 row[i] = g < 4 ? p.w_scales + (long long)min(row_of<GATED>(p, f0, g * 32 + lane), p.N - 1) * p.w_ld_scales
-                               : p.x_scales + (long long)min(t0 + (g - 4) * 32 + lane, p.M - 1) * p.x_ld_scales;
+                               : p.x_scales + (long long)min(t0 * PIECES + (g - 4) * 32 + lane, p.M * PIECES - 1) * p.x_ld_scales;
             }
             auto load = [&](int four, uint4 (&v)[MINE][2]) {          // 32 scales of each row, four chunks' worth; behind the last block 1
 #pragma unroll
@@ -213,10 +285,9 @@ rows4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
     __syncwarp();
     if (SPLIT && p.splits > 1) {
         pair_sync();                                 // every CTA's sums are in its shared memory
-        if (warp >= 2 && warp < 2 + EPI_WARPS) {
-            const int t0 = (first_tile % x_tiles) * BN, f0 = (first_tile / x_tiles) * OUTS;
-            join_splits<GATED>(p, smem_u32(stages), rank, min(BN, p.M - t0), t0, f0, outs, threadIdx.x - 64, 32 * EPI_WARPS);
-        }
+        const int t0 = (first_tile % x_tiles) * (BN / PIECES), f0 = (first_tile / x_tiles) * OUTS;
+        const auto again = [&](int l, int t) { return PIECES > 1 ? plain_dot(p, min(row_of<GATED>(p, f0, l), p.N - 1), t) : __int_as_float(0x7fffffff); };
+        join_splits<GATED>(p, smem_u32(stages), rank, min(BN / PIECES, p.M - t0), t0, f0, outs, threadIdx.x, THREADS, again);
         __syncwarp();
         pair_sync();                                 // nobody reads another CTA's sums any more
     }
@@ -232,13 +303,61 @@ rows4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
     }
 }
 
-template <bool GATED, int BN, int STAGES, bool SPLIT>
+// bfloat16 rows in eight pieces each: rows m * 8 + i of codes and scales.  Four lanes a block, eight numbers a lane.
+__global__ void __launch_bounds__(256) pieces_kernel(const __nv_bfloat16* __restrict__ x, long long ldx, uint32_t* __restrict__ codes,
+                                                     uint8_t* __restrict__ scales, int M, int K, int blocks, int ld_scales) {
+    chain_wait();
+    chain_release();
+    const int lanes = blocks * 4, total = M * lanes;
+    const int first = blockIdx.x * 256 + (threadIdx.x & ~31), at = first + (threadIdx.x & 31);
+    if (first >= total) return;                                       // a whole warp
+    const bool mine = at < total;
+    const int m = mine ? at / lanes : 0, part = mine ? at - m * lanes : 0;
+    float v[8];
+    if (mine && part * 8 < K) {                                       // K is a multiple of 8
+        const uint4 q = *reinterpret_cast<const uint4*>(x + (long long)m * ldx + part * 8);
+        const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[2 * i] = __uint_as_float(w[i] << 16), v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = 0.f;
+    }
+    for (int i = 0; i < PIECES8; ++i) {
+        uint32_t top = 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(v[e]) & 0x7fffffffu);       // what is not finite is largest
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const int exponent = (int)(top >> 23), s = exponent == 255 ? 255 : max(exponent - 2, 0);
+        uint32_t packed = 0;
+        if (exponent != 255) {
+            const float inverse = __uint_as_float((uint32_t)(254 - s) << 23), scale = mx_scale(s);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const uint32_t two = mx_codes_of_two(v[2 * e] * inverse, v[2 * e + 1] * inverse);
+                packed |= two << (8 * e);
+                v[2 * e] -= mx_code_value(two & 15) * scale;          // exact: both are multiples of the number's last bit or the code's
+                v[2 * e + 1] -= mx_code_value(two >> 4) * scale;
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = 0.f;                   // the first piece says NaN
+        }
+        if (mine) {
+            codes[((long long)m * PIECES8 + i) * lanes + part] = packed;
+            if ((part & 3) == 0) scales[((long long)m * PIECES8 + i) * ld_scales + (part >> 2)] = (uint8_t)s;
+        }
+    }
+}
+
+template <bool GATED, int BN, int STAGES, bool SPLIT, int PIECES = 1>
 int run(const void* x, long long ldx, MxParams& p, long long tiles, int sms, int device, cudaStream_t stream) {
     CUtensorMap map_w, map_x;
     if (make_codes_map<GATED>(&map_w, p)) return 1;
-    if (make_tile_map(&map_x, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, x, p.M, (long long)p.blocks * 16, ldx, BN, "gemm_mxfp4")) return 1;
+    if (make_tile_map(&map_x, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, x, (long long)p.M * PIECES, (long long)p.blocks * 16, ldx, BN, "gemm_mxfp4")) return 1;
     static unsigned long long allowed = 0;
-    return launch_mxfp4(rows4_kernel<GATED, BN, STAGES, SPLIT>, allowed, THREADS,
+    return launch_mxfp4(rows4_kernel<GATED, BN, STAGES, SPLIT, PIECES>, allowed, THREADS,
                         (size_t)STAGES * (A_BYTES + BN * ROW + 128 * scale_columns<BN>()) + 1024, SPLIT, tiles, sms, device, map_w, map_x, p, stream);
 }
 
@@ -246,20 +365,46 @@ template <bool GATED>
 int dispatch(const void* x, long long ldx, MxParams& p, cudaStream_t stream) {
     int sms = 148, device = 0;
     if (cudaGetDevice(&device) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
-    return cut_mxfp4<GATED, 192>(p, sms, [&](int bn, bool split, long long tiles) {
+    return cut_mxfp4<GATED, 192>(p, p.M, sms, [&](int bn, bool split, long long tiles) {
         if (bn == 256) return run<GATED, 256, 4, true>(x, ldx, p, tiles, sms, device, stream);
         if (bn == 192) return run<GATED, 192, 5, false>(x, ldx, p, tiles, sms, device, stream);
         if (bn == 128) return split ? run<GATED, 128, 6, true>(x, ldx, p, tiles, sms, device, stream)
                                     : run<GATED, 128, 6, false>(x, ldx, p, tiles, sms, device, stream);
-        if (bn == 64) return split ? run<GATED, 64, 8, true>(x, ldx, p, tiles, sms, device, stream)
-                                   : run<GATED, 64, 8, false>(x, ldx, p, tiles, sms, device, stream);
-        return split ? run<GATED, 32, 8, true>(x, ldx, p, tiles, sms, device, stream)
-                     : run<GATED, 32, 8, false>(x, ldx, p, tiles, sms, device, stream);
+        if (bn == 64) return run<GATED, 64, 4, true>(x, ldx, p, tiles, sms, device, stream);
+        return run<GATED, 32, 5, true>(x, ldx, p, tiles, sms, device, stream);
     });
+}
+
+template <bool GATED>
+int dispatch_pieces(const void* codes, MxParams& p, cudaStream_t stream) {
+    int sms = 148, device = 0;
+    if (cudaGetDevice(&device) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
+    const int rows = p.M * PIECES8, bn = rows <= 32 ? 32 : rows <= 64 ? 64 : rows <= 128 ? 128 : 256;
+    const long long ldx = (long long)p.blocks * 16;
+    const long long outs = GATED ? p.inter : p.N, per = GATED ? BM / 2 : BM, tiles = (outs + per - 1) / per * ((rows + bn - 1) / bn);
+    p.splits = splits_of(p, tiles, sms);
+    if (bn == 32) return run<GATED, 32, 5, true, PIECES8>(codes, ldx, p, tiles, sms, device, stream);
+    if (bn == 64) return run<GATED, 64, 4, true, PIECES8>(codes, ldx, p, tiles, sms, device, stream);
+    if (bn == 128) return run<GATED, 128, 6, true, PIECES8>(codes, ldx, p, tiles, sms, device, stream);
+    return run<GATED, 256, 4, true, PIECES8>(codes, ldx, p, tiles, sms, device, stream);
 }
 
 }  // namespace
 
 int mxfp4_rows4(const void* x, long long ldx, MxParams& p, int gated, cudaStream_t stream) {
     return gated ? dispatch<true>(x, ldx, p, stream) : dispatch<false>(x, ldx, p, stream);
+}
+
+long long mxfp4_pieces_bytes(int M, int blocks) { return (long long)M * PIECES8 * (blocks * 16 + (blocks + 15) / 16 * 16); }
+
+int mxfp4_pieces(const void* x, long long ldx, void* scratch, MxParams& p, int gated, cudaStream_t stream) {
+    uint8_t* codes = (uint8_t*)scratch;
+    uint8_t* scales = codes + (long long)p.M * PIECES8 * p.blocks * 16;
+    p.x_scales = scales;
+    p.x_ld_scales = (p.blocks + 15) / 16 * 16;
+    p.x16 = (const __nv_bfloat16*)x;
+    p.x16_ld = ldx;
+    TS_CHAINED_CHECK("gemm_mxfp4", launch_chained(pieces_kernel, dim3((p.M * p.blocks * 4 + 255) / 256), dim3(256), 0, stream, (const __nv_bfloat16*)x, ldx,
+                                                  (uint32_t*)codes, scales, p.M, p.K, p.blocks, (int)p.x_ld_scales));
+    return gated ? dispatch_pieces<true>(codes, p, stream) : dispatch_pieces<false>(codes, p, stream);
 }

@@ -14,12 +14,6 @@ namespace {
 
 constexpr int THREADS = 256;
 
-__device__ __forceinline__ uint32_t codes_of_two(float low, float high) {
-    uint32_t d;
-    asm("{\n\t.reg .b8 c;\n\tcvt.rn.satfinite.e2m1x2.f32 c, %1, %2;\n\tcvt.u32.u8 %0, c;\n\t}" : "=r"(d) : "f"(high), "f"(low));
-    return d;
-}
-
 template <typename T>
 __device__ __forceinline__ void load_eight(const T* p, int valid, bool wide, float (&v)[8]) {
     if (wide && valid >= 8) {
@@ -73,7 +67,7 @@ __global__ void __launch_bounds__(THREADS) quantize_mxfp4_kernel(const T* __rest
         uint32_t packed = 0;
         if (exponent != 255) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) packed |= codes_of_two(v[2 * i] * inverse, v[2 * i + 1] * inverse) << (8 * i);
+            for (int i = 0; i < 4; ++i) packed |= mx_codes_of_two(v[2 * i] * inverse, v[2 * i + 1] * inverse) << (8 * i);
         }
         if (mine) {
             codes[row * ld_codes + part] = packed;

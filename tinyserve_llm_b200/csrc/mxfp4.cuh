@@ -53,3 +53,12 @@ __device__ __forceinline__ uint32_t mx_mul(uint32_t a, uint32_t b) {
     asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
     return d;
 }
+
+// The codes of two numbers, the first in the lower four bits: the nearest, ties to the even code, magnitudes over 6 to 6.
+__device__ __forceinline__ uint32_t mx_codes_of_two(float low, float high) {
+    uint32_t d;
+    asm("{\n\t.reg .b8 c;\n\tcvt.rn.satfinite.e2m1x2.f32 c, %1, %2;\n\tcvt.u32.u8 %0, c;\n\t}" : "=r"(d) : "f"(high), "f"(low));
+    return d;
+}
+// The value of a code, by the same bits as above in a float32.
+__device__ __forceinline__ float mx_code_value(uint32_t code) { return __uint_as_float((code & 8) << 28 | (code & 7) << 22) * 0x1p126f; }

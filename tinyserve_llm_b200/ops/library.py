@@ -110,7 +110,8 @@ _SIGNATURES = {
     "ts_scale_tanh_cap": ("int", "plffp"),
     "ts_quantize_mxfp4": ("int", "ppplilllip"),
     "ts_dequantize_mxfp4": ("int", "ppplillip"),
-    "ts_gemm_mxfp4": ("int", "ppllplplp" "iiil" "iiffiipp"),
+    "ts_gemm_mxfp4": ("int", "ppllplplp" "iiil" "iiffipipp"),
+    "ts_gemm_mxfp4_scratch_bytes": ("long long", "iiii"),
 }
 _CTYPES = {"p": ctypes.c_void_p, "i": ctypes.c_int, "l": ctypes.c_longlong, "f": ctypes.c_float}
 _RETURNS = {"int": ctypes.c_int, "long long": ctypes.c_longlong, "void": None, "const char*": ctypes.c_char_p}
@@ -1762,9 +1763,15 @@ class Ops:
         if M == 0 or cols == 0:
             return out
         kind = 0 if activation is None else self.GATED_ACTIVATIONS[activation]
+        scratch = None
+        if not both:
+            size = self.lib.ts_gemm_mxfp4_scratch_bytes(M, N, K, 0)
+            if size:
+                scratch = torch.empty((size,), dtype=torch.uint8, device=rows.device)
+                self.launches += 1                           # the kernel that takes x apart
         self._call("ts_gemm_mxfp4", w.codes.data_ptr(), w.scales.data_ptr(), w.ld_codes, w.ld_scales, rows.data_ptr(), ldx, x_scales, x_ld_scales,
                    out.data_ptr(), M, N, K, cols, 0 if activation is None else 1, kind, limit, alpha, 1 if w.settled else 0,
-                   _DTYPE_CODE[out_dtype], self.error_word().data_ptr(), _stream())
+                   _ptr(scratch), _DTYPE_CODE[out_dtype], self.error_word().data_ptr(), _stream())
         return out
 
     def linear_columns(self, x: torch.Tensor, weight: torch.Tensor, out_dtype: torch.dtype | None = None) -> torch.Tensor:
