@@ -13,6 +13,7 @@ static bool few_in_registers(int M, int N, int K, bool both) {
 TS_API long long ts_gemm_mxfp4_scratch_bytes(int M, int N, int K, int both) {
     if (both || M <= 0 || N <= 0 || K <= 0) return 0;
     if (few_in_registers(M, N, K, both)) return 0;
+    if (K % 128) return 0;
     if (M > (getenv("MX_PIECES") ? atoi(getenv("MX_PIECES")) : 32)) return 0;
     return mxfp4_pieces_bytes(M, (K + MX_BLOCK - 1) / MX_BLOCK);
 }
@@ -40,7 +41,7 @@ TS_API int ts_gemm_mxfp4(const void* w_codes, const void* w_scales, long long w_
     MxParams p{(const uint8_t*)w_codes, (const uint8_t*)w_scales, w_ld_codes, w_ld_scales, (const uint8_t*)x_scales, x_ld_scales, y, ldy,
                M, N, K, blocks, N / 2, out_dtype == TS_F32 ? 1 : 0, act, limit, alpha, 0, nullptr, 0, settled, 1, error};
     const long long pieces = ts_gemm_mxfp4_scratch_bytes(M, N, K, x_scales != nullptr);
-    if (pieces) {
+    if (pieces && mxfp4_takes_pieces(w_codes, w_ld_codes, K)) {
         TS_REQUIRE(scratch && (uintptr_t)scratch % 16 == 0, "gemm_mxfp4: %lld bytes of scratch are needed", pieces);
         return mxfp4_pieces(x, ldx, scratch, p, gated, stream);
     }

@@ -41,7 +41,8 @@ struct MxParams {
 // Either form's products: the launcher's checks have been made.
 int mxfp4_rows16(const void* x, long long ldx, MxParams& p, int gated, cudaStream_t stream);
 int mxfp4_rows4(const void* x, long long ldx, MxParams& p, int gated, cudaStream_t stream);
-// A few rows in bfloat16 as pieces of four bits, which take `scratch`.
+// A few rows in bfloat16 as two pieces of eight bits, which take `scratch`.
+bool mxfp4_takes_pieces(const void* w_codes, long long w_ld_codes, int K);
 long long mxfp4_pieces_bytes(int M, int blocks);
 int mxfp4_pieces(const void* x, long long ldx, void* scratch, MxParams& p, int gated, cudaStream_t stream);
 
@@ -165,32 +166,30 @@ __device__ __forceinline__ void store_sixteen(const MxParams& p, const uint32_t 
 // W's codes of a chunk, 128 rows of 128 bytes; gated 16 gate rows, their up rows, and so on, which a map of four dimensions (bytes, 16
 // rows, halves, groups of 16 rows) brings in that order in one box.  Its groups have to be whole: else a box for every 16 rows.
 template <bool GATED>
-__device__ __forceinline__ void load_codes(unsigned char* to, const CUtensorMap* map, uint64_t* bar, const MxParams& p, int chunk, int f0) {
+__device__ __forceinline__ void load_codes(unsigned char* to, const CUtensorMap* map, uint64_t* bar, const MxParams& p, int column, int f0) {
     if (!GATED) {
-        tma_load_2d(to, map, bar, chunk * ROW, f0);
+        tma_load_2d(to, map, bar, column, f0);
     } else if (p.one_box) {
-        tma_load_4d(to, map, bar, chunk * ROW, 0, 0, f0 / 16);
+        tma_load_4d(to, map, bar, column, 0, 0, f0 / 16);
     } else {
 #pragma unroll
-        for (int g = 0; g < BM / 16; ++g) tma_load_2d(to + g * 16 * ROW, map, bar, chunk * ROW, row_of<true>(p, f0, g * 16));
+        for (int g = 0; g < BM / 16; ++g) tma_load_2d(to + g * 16 * ROW, map, bar, column, row_of<true>(p, f0, g * 16));
     }
 }
+// `spaced`: codes as elements of four bits, which TMA leaves 16 bytes for 16 of in shared memory, eight of them codes, as kind::mxf8f6f4 reads
+// them; else as they are, two in a byte.  Either way a box has 128 elements, and 128 bytes of shared memory, a row.
 template <bool GATED>
-int make_codes_map(CUtensorMap* map, MxParams& p) {
-    const long long bytes = (long long)p.blocks * 16;
-    if (!GATED || p.inter % 16 || p.inter / 16 < 4) {
-        p.one_box = 0;
-        return make_tile_map(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, p.w_codes, p.N, bytes, p.w_ld_codes, GATED ? 16 : BM, "gemm_mxfp4");
-    }
-    p.one_box = 1;
+int make_codes_map(CUtensorMap* map, MxParams& p, bool spaced = false) {
     EncodeTiled encode = encode_tiled();
     if (!encode) return ts_fail("gemm_mxfp4: the driver does not export cuTensorMapEncodeTiled");
-    const cuuint64_t dims[4] = {(cuuint64_t)bytes, 16, 2, (cuuint64_t)p.inter / 16};
-    const cuuint64_t strides[3] = {(cuuint64_t)p.w_ld_codes, (cuuint64_t)p.w_ld_codes * p.inter, (cuuint64_t)p.w_ld_codes * 16};
-    const cuuint32_t box[4] = {ROW, 16, 2, 4}, elem[4] = {1, 1, 1, 1};
-    const CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<uint8_t*>(p.w_codes), dims, strides, box, elem,
-                              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
-                              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    const CUtensorMapDataType type = spaced ? CU_TENSOR_MAP_DATA_TYPE_16U4_ALIGN16B : CU_TENSOR_MAP_DATA_TYPE_UINT8;
+    const cuuint64_t elements = (cuuint64_t)p.blocks * (spaced ? 32 : 16), ld = (cuuint64_t)p.w_ld_codes;
+    p.one_box = GATED && p.inter % 16 == 0 && p.inter / 16 >= 4;
+    const cuuint64_t dims[4] = {elements, p.one_box ? 16ull : (cuuint64_t)p.N, 2, (cuuint64_t)p.inter / 16};
+    const cuuint64_t strides[3] = {ld, ld * p.inter, ld * 16};
+    const cuuint32_t box[4] = {128, GATED ? 16u : (cuuint32_t)BM, 2, 4}, elem[4] = {1, 1, 1, 1};
+    const CUresult r = encode(map, type, p.one_box ? 4 : 2, const_cast<uint8_t*>(p.w_codes), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) return ts_fail("gemm_mxfp4: cuTensorMapEncodeTiled failed with %d", (int)r);
     return 0;
 }

@@ -8,8 +8,10 @@
 
 namespace {
 
-// Warps: producer of x, issuer, four of the epilogue, one that brings codes, four teams of four that spread them.
-constexpr int EPI_WARPS = 4, TEAMS = 4, TEAM = 4, THREADS = 32 * (3 + EPI_WARPS + TEAMS * TEAM);
+// Warps: producer of x, issuer, four of the epilogue, one that brings codes, teams of four that spread them: four teams, or two where tiles
+// are small and two CTAs share an SM, one's beginning and end beside the other's stream of W.
+constexpr int EPI_WARPS = 4, TEAM = 4;
+constexpr int threads_of(int teams) { return 32 * (3 + EPI_WARPS + teams * TEAM); }
 constexpr int BK = 64, PER_CHUNK = CHUNK / BK, STAGE_COLS = BK / 2;    // a stage's columns of K; of tensor memory
 
 __device__ __forceinline__ void umma(uint32_t leader, uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
@@ -28,12 +30,13 @@ __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&r)[16]
 }
 
 // BN: rows of x a tile.  STAGES: x's ring.  PACKED: chunks of codes in shared memory.  MADE: stages of numbers in tensor memory.
-template <bool GATED, int BN, int STAGES, int PACKED, bool SPLIT>
-__global__ void __launch_bounds__(THREADS, 1)
+template <bool GATED, int BN, int STAGES, int PACKED, bool SPLIT, int TEAMS>
+__global__ void __launch_bounds__(32 * (3 + EPI_WARPS + TEAMS * TEAM), TEAMS == 2 ? 2 : 1)
 rows16_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, MxParams p) {
     constexpr int B_BYTES = BN * ROW, ACCUMULATORS = SPLIT ? 1 : 2, OUTS = GATED ? BM / 2 : BM, SHARE = BN / (EPI_WARPS / 4);
-    constexpr int MADE = STAGES < 8 || (512 - ACCUMULATORS * BN) / STAGE_COLS < 8 ? 4 : 8, TMEM_COLS = power_of_two(ACCUMULATORS * BN + MADE * STAGE_COLS);
-    static_assert(ACCUMULATORS * BN + MADE * STAGE_COLS <= 512, "tensor memory has 512 columns");
+    constexpr int THREADS = 32 * (3 + EPI_WARPS + TEAMS * TEAM);
+    constexpr int MADE = STAGES < 8 || TEAMS == 2 || (512 - ACCUMULATORS * BN) / STAGE_COLS < 8 ? 4 : 8, TMEM_COLS = power_of_two(ACCUMULATORS * BN + MADE * STAGE_COLS);
+    static_assert(TMEM_COLS * (TEAMS == 2 ? 2 : 1) <= 512 && ACCUMULATORS * BN + MADE * STAGE_COLS <= TMEM_COLS, "tensor memory has 512 columns");
     static_assert(STAGES >= MADE, "a stage's barriers go round once more only after its place in tensor memory has been waited for");
     static_assert(!SPLIT || BM * BN * 4 <= STAGES * B_BYTES, "a split tile's sums go where the ring was");
     extern __shared__ __align__(1024) unsigned char smem_raw[];
@@ -147,7 +150,7 @@ rows16_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
                 for (int chunk = chunk0; chunk < chunk1; ++chunk, b.next()) {
                     if (!wait_for(&packed_empty[b.at], b.parity ^ 1, p.error, 47)) { failed = 1; break; }
                     mbar_expect_tx(&packed_full[b.at], A_BYTES);
-                    load_codes<GATED>(packed_ring + b.at * A_BYTES, &map_w, &packed_full[b.at], p, chunk, f0);
+                    load_codes<GATED>(packed_ring + b.at * A_BYTES, &map_w, &packed_full[b.at], p, chunk * ROW, f0);
                 }
             }
         }
@@ -155,8 +158,8 @@ rows16_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
         if (codes_first) chain_wait();
     } else {
         // ---------------------------------------------------------------- codes to bfloat16 numbers
-        // Team j makes quarter j of every chunk, one stage, so that four stages are in the making at a time; a thread takes the row of its lane
-        // of tensor memory and both blocks of its quarter.  Eight lanes that read shared memory together have eight neighbouring rows, whose
+        // Team j makes quarter j of every chunk (of two teams each makes two), one stage, so that as many stages are in the making at a time; a
+        // thread takes the row of its lane of tensor memory and both blocks of its quarter.  Eight lanes that read shared memory together have eight neighbouring rows, whose
         // 16-byte pieces the swizzle puts into different banks.
         const int team = (warp - 3 - EPI_WARPS) / TEAM, l = (warp & 3) * 32 + lane;
         const uint32_t to = tmem_made + ((uint32_t)((warp & 3) * 32) << 16);
@@ -181,53 +184,58 @@ rows16_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
                 return v;
             };
             uint4 now = load_scales(chunk0 >> 1), next = make_uint4(0, 0, 0, 0);
-            for (int chunk = chunk0; chunk < chunk1; ++chunk, b.next(), kg += PER_CHUNK) {
-                const int m = kg % MADE;
+            for (int chunk = chunk0; chunk < chunk1 && ok; ++chunk, b.next()) {
                 if (!(chunk & 1) || chunk == chunk0) next = load_scales((chunk >> 1) + 1);
                 ok = __all_sync(0xffffffffu, wait_for(&packed_full[b.at], b.parity, p.error, 48) && !failed);
                 if (!ok) { failed = 1; break; }
-                uint4 code[2];
 #pragma unroll
-                for (int part = 0; part < 2; ++part)
-                    code[part] = *reinterpret_cast<const uint4*>(packed_ring + b.at * A_BYTES + l * ROW + (((team * 2 + part) ^ (l & 7)) << 4));
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&packed_empty[b.at]);
-                const uint32_t four = chunk & 1 ? (team & 2 ? now.w : now.z) : (team & 2 ? now.y : now.x);
-                const uint32_t sc = team & 1 ? four >> 16 : four & 0xffff;
-                const bool large = __any_sync(0xffffffffu, max(sc & 255, sc >> 8) > 128);
-                if (kg >= MADE) {
-                    const int before = kg - MADE;
-                    ok = __all_sync(0xffffffffu, wait_for(&empty_bar[before % STAGES], (before / STAGES) & 1, p.error, 46) && !failed);
-                    if (!ok) { failed = 1; break; }
-                }
-                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                for (int quarter = team; quarter < PER_CHUNK; quarter += TEAMS, kg += TEAMS) {
+                    const int m = kg % MADE;
+                    uint4 code[2];
 #pragma unroll
-                for (int part = 0; part < 2; ++part) {
-                    const uint32_t w[4] = {code[part].x, code[part].y, code[part].z, code[part].w};
-                    const uint32_t scale = part ? sc >> 8 : sc & 255;
-                    uint32_t q[16];
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        uint32_t four_of[4];
-                        mx_spread_neighbours(w[j], four_of);
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) q[4 * j + e] = four_of[e];
+                    for (int part = 0; part < 2; ++part)
+                        code[part] = *reinterpret_cast<const uint4*>(packed_ring + b.at * A_BYTES + l * ROW + (((quarter * 2 + part) ^ (l & 7)) << 4));
+                    if (quarter + TEAMS >= PER_CHUNK) {
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&packed_empty[b.at]);
                     }
-                    if (!large) {
-                        const uint32_t factor = mx_factor(scale);
-#pragma unroll
-                        for (int e = 0; e < 16; ++e) q[e] = mx_mul(q[e], factor);
-                    } else {
-                        const MxFactor two = mx_factor_large(scale);
-#pragma unroll
-                        for (int e = 0; e < 16; ++e) q[e] = mx_mul(mx_mul(q[e], two.first), two.more);
+                    const uint32_t four = chunk & 1 ? (quarter & 2 ? now.w : now.z) : (quarter & 2 ? now.y : now.x);
+                    const uint32_t sc = quarter & 1 ? four >> 16 : four & 0xffff;
+                    const bool large = __any_sync(0xffffffffu, max(sc & 255, sc >> 8) > 128);
+                    if (kg >= MADE) {
+                        const int before = kg - MADE;
+                        ok = __all_sync(0xffffffffu, wait_for(&empty_bar[before % STAGES], (before / STAGES) & 1, p.error, 46) && !failed);
+                        if (!ok) { failed = 1; break; }
                     }
-                    tmem_st16(to + m * STAGE_COLS + part * 16, q);
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll
+                    for (int part = 0; part < 2; ++part) {
+                        const uint32_t w[4] = {code[part].x, code[part].y, code[part].z, code[part].w};
+                        const uint32_t scale = part ? sc >> 8 : sc & 255;
+                        uint32_t q[16];
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            uint32_t four_of[4];
+                            mx_spread_neighbours(w[j], four_of);
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) q[4 * j + e] = four_of[e];
+                        }
+                        if (!large) {
+                            const uint32_t factor = mx_factor(scale);
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) q[e] = mx_mul(q[e], factor);
+                        } else {
+                            const MxFactor two = mx_factor_large(scale);
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) q[e] = mx_mul(mx_mul(q[e], two.first), two.more);
+                        }
+                        tmem_st16(to + m * STAGE_COLS + part * 16, q);
+                    }
+                    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&full_bar[kg % STAGES]);
                 }
-                asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&full_bar[kg % STAGES]);
                 if (chunk & 1) now = next;
             }
         }
@@ -253,14 +261,14 @@ rows16_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
     }
 }
 
-template <bool GATED, int BN, int STAGES, int PACKED, bool SPLIT>
+template <bool GATED, int BN, int STAGES, int PACKED, bool SPLIT, int TEAMS>
 int run(const void* x, long long ldx, MxParams& p, long long tiles, int sms, int device, cudaStream_t stream) {
     CUtensorMap map_w, map_x;
     if (make_codes_map<GATED>(&map_w, p)) return 1;
     if (make_tile_map(&map_x, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, x, p.M, p.K, ldx, BN, "gemm_mxfp4")) return 1;
     static unsigned long long allowed = 0;
-    return launch_mxfp4(rows16_kernel<GATED, BN, STAGES, PACKED, SPLIT>, allowed, THREADS, (size_t)STAGES * BN * ROW + PACKED * A_BYTES + 1024, SPLIT,
-                        tiles, sms, device, map_w, map_x, p, stream);
+    return launch_mxfp4(rows16_kernel<GATED, BN, STAGES, PACKED, SPLIT, TEAMS>, allowed, threads_of(TEAMS),
+                        (size_t)STAGES * BN * ROW + PACKED * A_BYTES + 1024, SPLIT, tiles, sms, device, map_w, map_x, p, stream);
 }
 
 template <bool GATED>
@@ -268,14 +276,12 @@ int dispatch(const void* x, long long ldx, MxParams& p, cudaStream_t stream) {
     int sms = 148, device = 0;
     if (cudaGetDevice(&device) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
     return cut_mxfp4<GATED, 192>(p, p.M, sms, [&](int bn, bool split, long long tiles) {
-        if (bn == 256) return run<GATED, 256, 5, 3, true>(x, ldx, p, tiles, sms, device, stream);
-        if (bn == 192) return run<GATED, 192, 6, 4, false>(x, ldx, p, tiles, sms, device, stream);
-        if (bn == 128) return split ? run<GATED, 128, 8, 4, true>(x, ldx, p, tiles, sms, device, stream)
-                                    : run<GATED, 128, 8, 4, false>(x, ldx, p, tiles, sms, device, stream);
-        if (bn == 64) return split ? run<GATED, 64, 8, 6, true>(x, ldx, p, tiles, sms, device, stream)
-                                   : run<GATED, 64, 8, 6, false>(x, ldx, p, tiles, sms, device, stream);
-        return split ? run<GATED, 32, 8, 6, true>(x, ldx, p, tiles, sms, device, stream)
-                     : run<GATED, 32, 8, 6, false>(x, ldx, p, tiles, sms, device, stream);
+        if (bn == 256) return run<GATED, 256, 5, 3, true, 4>(x, ldx, p, tiles, sms, device, stream);
+        if (bn == 192) return run<GATED, 192, 6, 4, false, 4>(x, ldx, p, tiles, sms, device, stream);
+        if (bn == 128) return split ? run<GATED, 128, 4, 2, true, 2>(x, ldx, p, tiles, sms, device, stream)
+                                    : run<GATED, 128, 8, 4, false, 4>(x, ldx, p, tiles, sms, device, stream);
+        if (bn == 64) return run<GATED, 64, 6, 3, true, 2>(x, ldx, p, tiles, sms, device, stream);
+        return run<GATED, 32, 8, 4, true, 2>(x, ldx, p, tiles, sms, device, stream);
     });
 }
 

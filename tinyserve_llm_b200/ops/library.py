@@ -147,6 +147,7 @@ _WAIT_CODES: dict[int, tuple[str, str]] = {
     43: ("gemm_mxfp4", "epilogue waiting for an accumulator"),
     44: ("gemm_mxfp4", "MMA issuer waiting for a drained accumulator"),
     45: ("gemm_mxfp4", "warps of the scales waiting for a free ring slot"),
+    49: ("gemm_mxfp4", "MMA issuer waiting for scales"),
     46: ("gemm_mxfp4", "warps that spread codes waiting for free tensor memory"),
     47: ("gemm_mxfp4", "TMA producer of codes waiting for a free buffer"),
     48: ("gemm_mxfp4", "warps that spread codes waiting for a chunk of them"),
