@@ -38,6 +38,10 @@ def build_parser() -> argparse.ArgumentParser:
     p.add_argument("--ignore-eos", action="store_true")
     p.add_argument("--seed", type=int, default=0)
     p.add_argument("--dtype", choices=["bfloat16", "float32"], default="bfloat16")
+    p.add_argument("--weight-format", choices=["mxfp4"], default=None,
+                   help="hold the projections' weights in microscaled 4-bit floating point")
+    p.add_argument("--activation-format", choices=["mxfp4"], default=None,
+                   help="round the rows those weights multiply to four bits as well")
     p.add_argument("--block-size", type=int, default=256, help="tokens per cache page")
     p.add_argument("--num-blocks", type=int, default=None, help="cache pages; default: sized from free memory")
     p.add_argument("--gpu-memory-utilization", type=float, default=0.9)
@@ -73,8 +77,11 @@ def main(argv: list[str] | None = None) -> int:
     started = time.time()
     llm = LLM(args.model, scheduler_config, cache_config, dtype=args.dtype, num_blocks=args.num_blocks,
               gpu_memory_utilization=args.gpu_memory_utilization, seed=args.seed,
-              random_weights_seed=args.random_weights)
-    print(f"model {args.model} ({args.dtype}); cache {llm.cache.num_pages} pages of {args.block_size} tokens; "
+              random_weights_seed=args.random_weights, weight_format=args.weight_format,
+              activation_format=args.activation_format)
+    held = f", weights {args.weight_format}" if args.weight_format else ""
+    held += f", activations {args.activation_format}" if args.activation_format else ""
+    print(f"model {args.model} ({args.dtype}{held}); cache {llm.cache.num_pages} pages of {args.block_size} tokens; "
           f"{len(prompts)} prompts", flush=True)
     params = SamplingParams(max_tokens=args.max_tokens, temperature=args.temperature, n=args.n,
                             ignore_eos=args.ignore_eos)
@@ -93,6 +100,8 @@ def main(argv: list[str] | None = None) -> int:
             "engine": "tinyserve_llm_b200",
             "model": args.model,
             "dtype": args.dtype,
+            "weight_format": args.weight_format,
+            "activation_format": args.activation_format,
             "caching": args.caching,
             "temperature": args.temperature,
             "seed": args.seed,

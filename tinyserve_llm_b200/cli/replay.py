@@ -3,6 +3,7 @@ Trace replay: feeds given token ids through a model step by step and writes the 
 
     bin/trace_run --model DIR --dtype bfloat16|float32 --out DIR --max-tokens N
                   [--page-tokens 64] [--max-requests 4] [--caching off|on]
+                  [--weight-format mxfp4 [--activation-format mxfp4]]
 
 Steps come on standard input, one JSON object a line:
 
@@ -48,6 +49,10 @@ def main(argv: list[str] | None = None) -> int:
                         help="most requests live at any time: the state slots of models that keep per-request state (default 4)")
     parser.add_argument("--caching", choices=["on", "off"], default="off",
                         help="on: ended requests' pages stay indexed and new requests reuse them")
+    parser.add_argument("--weight-format", choices=["mxfp4"], default=None,
+                        help="hold the projections' weights in microscaled 4-bit floating point")
+    parser.add_argument("--activation-format", choices=["mxfp4"], default=None,
+                        help="round the rows those weights multiply to four bits as well")
     args = parser.parse_args(argv)
     if args.page_tokens <= 0:
         parser.error("--page-tokens must be positive")
@@ -58,7 +63,7 @@ def main(argv: list[str] | None = None) -> int:
     from tinyserve_llm_b200.engine.step import StepEntry, StepRunner
 
     os.makedirs(args.out, exist_ok=True)
-    model = load_model(args.model, args.dtype, "cuda")
+    model = load_model(args.model, args.dtype, "cuda", weight_format=args.weight_format, activation_format=args.activation_format)
     num_pages = max(1, -(-args.max_tokens // args.page_tokens))
     _, manager, storage = build_cache(model, args.page_tokens, num_pages, caching=args.caching == "on",
                                       num_state_slots=max(1, args.max_requests))

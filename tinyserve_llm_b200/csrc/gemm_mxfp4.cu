@@ -1,20 +1,24 @@
 // The launcher of the products over microscaled 4-bit weights (gemm_mxfp4.cuh): checks of the arguments.
 #include "gemm_mxfp4.cuh"
 #include "skinny_mxfp4.h"
-#include <cstdlib>
 
-// Whether a few rows go by the kernel that spreads codes in registers.
+// Whether a few rows go by the kernel that spreads codes in registers: no kernel has less between its launch and its end, but it takes a
+// cycle for every 13 numbers of W and SM.  Measured on a B200 (graphs of different weights): 2,048 by 2,048, 1 to 16 rows in bfloat16 2.9 to
+// 4.1 us (in pieces 7.2 to 8.0), in four bits 3.1 to 3.7 (tcgen05 4.4 to 5.1); 2,048 by 8,192, 1 to 8 rows in bfloat16 8.1 to 9.0 (9.2 to
+// 10.0), 16 rows 11.7 (10.2); 16,384 by 2,048, 8 rows 13.2 (10.7).
 static bool few_in_registers(int M, int N, int K, bool both) {
-    if (getenv("MX_FEW")) return M <= atoi(getenv("MX_FEW"));
-    return M <= SKINNY_MX_ROWS;
+    const long long numbers = (long long)N * K;
+    return (M <= SKINNY_MX_ROWS && numbers <= 5ll << 20) || (!both && M <= 8 && numbers <= 1ll << 24);
 }
 
-// Bytes of scratch a product needs (16-byte aligned; 0: none): rows in bfloat16 that are worked on in pieces.
+// Whether rows in bfloat16 are multiplied as two rows of 8-bit numbers each, with W's codes as they are, and not with W's codes spread to
+// bfloat16: 28,672 by 4,096 gated, 8 rows 18.4 us (spread 40.7), 64 rows 28 (42.6), 96 rows 56 (46); 2,048 by 8,192, 17 to 64 rows 10.3 to
+// 14.0 (13.9 to 15.5); 2,048 by 2,048, 64 rows 9.7 (9.0).
+static bool in_pieces(int M, int N, int K) { return K % 128 == 0 && M <= 64 && (long long)N * K > 5ll << 20; }
+
+// Bytes of scratch a product may need (16-byte aligned; 0: none).
 TS_API long long ts_gemm_mxfp4_scratch_bytes(int M, int N, int K, int both) {
-    if (both || M <= 0 || N <= 0 || K <= 0) return 0;
-    if (few_in_registers(M, N, K, both)) return 0;
-    if (K % 128) return 0;
-    if (M > (getenv("MX_PIECES") ? atoi(getenv("MX_PIECES")) : 32)) return 0;
+    if (both || M <= 0 || N <= 0 || K <= 0 || few_in_registers(M, N, K, false) || !in_pieces(M, N, K)) return 0;
     return mxfp4_pieces_bytes(M, (K + MX_BLOCK - 1) / MX_BLOCK);
 }
 

@@ -327,7 +327,9 @@ int cut_mxfp4(MxParams& p, int rows, int sms, const Run& run) {
     p.splits = 1;
     if (rows > 128) {
         if (tiles_of(256) <= sms && tiles_of(256) * 4 >= 3ll * sms) return run(256, true, tiles_of(256));
-        if (tiles_of(WIDE) > sms) return run(WIDE, false, tiles_of(WIDE));
+        // wide tiles or narrow ones, by the rounds they take and what a tile costs beside its columns
+        auto cost = [&](int bn) { return (tiles_of(bn) + sms - 1) / sms * (bn + 128); };
+        if (tiles_of(WIDE) > sms && cost(WIDE) <= cost(128)) return run(WIDE, false, tiles_of(WIDE));
     }
     const int bn = rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
     const long long tiles = tiles_of(bn);

@@ -4,7 +4,8 @@ The Python entry point: LLM(model_path).generate(prompts, SamplingParams(...)).
 Names and meanings of the options follow tinyserve-llm (engine/llm_engine.py:66-185,
 engine/interface.py:28-32): SchedulerConfig, CacheConfig(block_size, caching, device), dtype,
 num_blocks (None: sized from free device memory after a warm-up step), gpu_memory_utilization, seed,
-load_tokenizer; add_request / step / generate; Completion and StepRecord.  There is no `attention`
+load_tokenizer; add_request / step / generate; Completion and StepRecord.  `weight_format` and `activation_format` ("mxfp4"): weights, and
+the rows they multiply, in microscaled 4-bit floating point (engine/loading.py says which).  There is no `attention`
 option: the engine has one attention implementation, its own kernels.  New here: `cuda_graphs` and
 `run_ahead` (decode steps launched before the previous step's samples have reached the host).
 """
@@ -94,13 +95,16 @@ class LLM:
             seed: int | None = None,
             load_tokenizer: bool | None = None,
             random_weights_seed: int | None = None,
+            weight_format: str | None = None,
+            activation_format: str | None = None,
             cuda_graphs: bool = True,
             run_ahead: bool = True,
     ) -> None:
         self.device = require_cuda(cache_config.device)
         self.dtype = resolve_dtype(dtype)
         torch.cuda.set_device(self.device)
-        self.model = load_model(model_path, self.dtype, self.device, random_weights_seed=random_weights_seed)
+        self.model = load_model(model_path, self.dtype, self.device, random_weights_seed=random_weights_seed,
+                                weight_format=weight_format, activation_format=activation_format)
         spec = self.model.spec
         if scheduler_config.max_model_len > spec.max_positions:
             raise ValueError(f"max_model_len = {scheduler_config.max_model_len} exceeds the model's "

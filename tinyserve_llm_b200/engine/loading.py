@@ -42,16 +42,36 @@ def require_cuda(device: str | torch.device = "cuda") -> torch.device:
     return device
 
 
+FORMATS = (None, "mxfp4")
+
+
+def check_formats(weight_format: str | None, activation_format: str | None, dtype: torch.dtype) -> None:
+    """What a model's weights, and the rows they multiply, may be held in: as they come, or in microscaled 4-bit floating point."""
+    for value, name in ((weight_format, "weight_format"), (activation_format, "activation_format")):
+        if value not in FORMATS:
+            raise ValueError(f"{name} must be one of {FORMATS}, got {value!r}")
+    if weight_format is not None and dtype != torch.bfloat16:
+        raise ValueError(f"weight_format={weight_format!r} needs dtype bfloat16, got {dtype}")
+    if activation_format is not None and weight_format is None:
+        raise ValueError("activation_format needs a weight_format: only 4-bit weights multiply 4-bit rows")
+
+
 def load_model(model_dir: str, dtype: str | torch.dtype = "bfloat16", device: str | torch.device = "cuda", *,
-               random_weights_seed: int | None = None) -> DecoderModel:
+               random_weights_seed: int | None = None, weight_format: str | None = None,
+               activation_format: str | None = None) -> DecoderModel:
     """
     The model of the folder, chosen by its config.json.  With `random_weights_seed` the folder needs
     only config.json: every declared tensor is drawn instead of read, with the generator and in the
     dtype `write_random_model` uses, so that one seed gives one model whichever way it is made (the
     draws run on the host, about ten seconds per billion weights, and go to the device tensor by tensor).
+
+    `weight_format="mxfp4"`: the projections of attention (the paged grouped-query kind) and of dense feed-forwards are rounded to
+    microscaled 4-bit floating point and kept in it; embedding, vocabulary projection, norms and every other kind of mixer stay as they
+    are.  `activation_format="mxfp4"`: the rows those projections multiply are rounded to four bits as well.
     """
-    device = require_cuda(device)
     dtype = resolve_dtype(dtype)
+    check_formats(weight_format, activation_format, dtype)
+    device = require_cuda(device)
     _, spec = load_model_spec(model_dir)
     declared = declared_tensors(spec)
     if random_weights_seed is None:
@@ -60,7 +80,11 @@ def load_model(model_dir: str, dtype: str | torch.dtype = "bfloat16", device: st
     else:
         tensors = {name: t.to(device) for name, t in random_tensors(declared, random_weights_seed, dtype=torch.bfloat16)}
     with torch.cuda.device(device):
-        return DecoderModel(spec, tensors, Runtime(dtype=dtype, device=device, ops=get_ops()))
+        rt = Runtime(dtype=dtype, device=device, ops=get_ops(), weight_format=weight_format, activation_format=activation_format)
+        model = DecoderModel(spec, tensors, rt)
+    if weight_format is not None and not rt.shared.get("quantized_bytes"):
+        raise ValueError(f"weight_format={weight_format!r}: no part of this model holds its weights in that form")
+    return model
 
 
 def build_cache(model: DecoderModel, page_tokens: int, num_pages: int, *, caching: bool = True,

@@ -1755,7 +1755,7 @@ class Ops:
         self._check_here(rows, "x")
         cols = N if activation is None else N // 2
         if out is None:
-            out = torch.empty((M, cols), dtype=out_dtype, device=rows.device)
+            out = rows.new_empty((M, cols)) if rows.dtype is out_dtype else rows.new_empty((M, cols), dtype=out_dtype)
         else:
             self._check(out, "out", out_dtype, 2)
             self._check_here(out, "out")
@@ -1765,7 +1765,7 @@ class Ops:
             return out
         kind = 0 if activation is None else self.GATED_ACTIVATIONS[activation]
         scratch = None
-        if not both:
+        if not both and M <= 64:
             size = self.lib.ts_gemm_mxfp4_scratch_bytes(M, N, K, 0)
             if size:
                 scratch = torch.empty((size,), dtype=torch.uint8, device=rows.device)

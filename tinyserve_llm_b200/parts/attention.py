@@ -14,7 +14,7 @@ import torch
 
 from tinyserve_llm_b200.config.spec import AttentionSpec
 from tinyserve_llm_b200.parts.base import KVNeed, Mixer, Runtime, TensorDecl, part_class, register_part
-from tinyserve_llm_b200.parts.linear import Linear, fuse_rows
+from tinyserve_llm_b200.parts.linear import QuantizedLinear, fuse_rows, projection
 
 
 MAX_HEAD_DIM = 256      # csrc/attention_generic.cu, the kernel every size falls back to
@@ -48,9 +48,9 @@ class PagedAttention(Mixer):
     def __init__(self, spec: AttentionSpec, tensors: dict[str, torch.Tensor], rt: Runtime) -> None:
         super().__init__(spec, tensors, rt)
         self.validate(spec)
-        self.qkv = Linear(fuse_rows([tensors["q_proj.weight"], tensors["k_proj.weight"],
-                                     tensors["v_proj.weight"]]), rt)
-        self.out = Linear(tensors["o_proj.weight"], rt)
+        self.qkv = projection(fuse_rows([tensors["q_proj.weight"], tensors["k_proj.weight"],
+                                         tensors["v_proj.weight"]]), rt)
+        self.out = projection(tensors["o_proj.weight"], rt)
         self.position = None
         if spec.position is not None:
             self.position = part_class("position", spec.position)(spec.position, {}, rt)
@@ -62,7 +62,8 @@ class PagedAttention(Mixer):
         spec, ops = self.spec, self.rt.ops
         table = self.position.table if self.position is not None else None
         qkv = None
-        if self.position is None or table is not None:          # a few tokens: projection, rotation and cache write in one kernel
+        fused = not isinstance(self.qkv, QuantizedLinear)
+        if fused and (self.position is None or table is not None):          # a few tokens: projection, rotation and cache write in one kernel
             qkv = ops.linear_rope_store(x, self.qkv.weight, ctx, binding, table, spec.num_heads, spec.num_kv_heads,
                                         spec.head_dim)
         if qkv is None:

@@ -46,6 +46,8 @@ class Runtime:
     device: torch.device
     ops: Any                  # tinyserve_llm_b200.ops.Ops
     shared: dict = field(default_factory=dict)   # buffers parts of one model share (position tables)
+    weight_format: str | None = None      # "mxfp4": projections that come in that form hold their weights in four bits
+    activation_format: str | None = None  # "mxfp4": and round the rows they multiply to four bits as well
 
 
 class Part:

@@ -15,7 +15,7 @@ import torch
 
 from tinyserve_llm_b200.config.spec import GatedMLPSpec, PlainMLPSpec
 from tinyserve_llm_b200.parts.base import FeedForward, Runtime, TensorDecl, register_part
-from tinyserve_llm_b200.parts.linear import Linear, fuse_rows
+from tinyserve_llm_b200.parts.linear import fuse_rows, projection
 
 
 @register_part("feed_forward", "gated_mlp")
@@ -38,13 +38,13 @@ class GatedMLP(FeedForward):
         if spec.activation not in self.ACTIVATIONS:
             raise NotImplementedError(f"activation {spec.activation!r} is not supported; have {self.ACTIVATIONS}")
         gate, up, down = spec.tensor_names
-        self.gate_up = Linear(fuse_rows([tensors[gate], tensors[up]]), rt)
-        self.down = Linear(tensors[down], rt)
+        self.gate_up = projection(fuse_rows([tensors[gate], tensors[up]]), rt)
+        self.down = projection(tensors[down], rt)
 
     def forward(self, x: torch.Tensor, ctx) -> torch.Tensor:
-        spec, ops = self.spec, self.rt.ops
+        spec = self.spec
         # the gate/up products carry the activation in their epilogue where there is a kernel of the engine's own for the size
-        return self.down(ops.linear_gated(x, self.gate_up.weight, spec.activation, spec.limit, spec.alpha))
+        return self.down(self.gate_up.gated(x, spec.activation, spec.limit, spec.alpha))
 
 
 @register_part("feed_forward", "plain_mlp")
@@ -76,8 +76,8 @@ class PlainMLP(FeedForward):
         if spec.activation not in self.ACTIVATIONS:
             raise NotImplementedError(f"activation {spec.activation!r} is not supported; have {self.ACTIVATIONS}")
         up, down = spec.tensor_names
-        self.up = Linear(tensors[up], rt)
-        self.down = Linear(tensors[down], rt)
+        self.up = projection(tensors[up], rt)
+        self.down = projection(tensors[down], rt)
         self.factors = (0.0, 0.0)
         if spec.activation == "xielu":
             p, q = (float(v) for v in tensors[spec.param_name].to(torch.float64).cpu().tolist())
@@ -86,4 +86,4 @@ class PlainMLP(FeedForward):
 
     def forward(self, x: torch.Tensor, ctx) -> torch.Tensor:
         # a few rows: the activation rides in the up product's epilogue; more: the library's product, then one pass
-        return self.down(self.rt.ops.linear_unary(x, self.up.weight, self.spec.activation, *self.factors))
+        return self.down(self.up.unary(x, self.spec.activation, *self.factors))
