@@ -227,6 +227,7 @@ class Ops:
         # TINYSERVE_B200_TILES=0 keeps the recurrences that have a form of sixteen tokens at a time on the scan token by token
         self.recurrence_tiles = os.environ.get("TINYSERVE_B200_TILES", "1") != "0"
         self._tile_floats: dict[tuple[int, int, int, int], tuple[int, int]] = {}   # sizes of a tile's buffers
+        self._scratch_mxfp4: dict[tuple[int, int, int], int] = {}                   # bytes of scratch of a product over 4-bit weights
         # TINYSERVE_B200_OVERLAP=0 keeps a replayed step's kernels on one stream (see parts/overlap.py)
         self.overlap = os.environ.get("TINYSERVE_B200_OVERLAP", "1") != "0"
         # TINYSERVE_B200_LRU=split keeps a gated linear recurrent unit's decode steps on the kernels of prompt portions
@@ -1715,8 +1716,9 @@ class Ops:
         [M, K], K a multiple of 8, rows contiguous or stretches of wider rows that start 16-byte aligned; or rows quantised like the weight
         (any K): then both sides stay in four bits.  Sums in float32, rounded once.  `out` (contiguous, of the output dtype) receives the product.
         """
-        out_dtype = out_dtype or torch.bfloat16
-        if out_dtype not in _DTYPE_CODE:
+        if out_dtype is None:
+            out_dtype = torch.bfloat16
+        elif out_dtype not in _DTYPE_CODE:
             raise KernelError(f"linear_mxfp4: output dtype {out_dtype}, expected one of {tuple(_DTYPE_CODE)}")
         return self._product_mxfp4("linear_mxfp4", x, weight, None, 0.0, 1.0, out_dtype, out)
 
@@ -1734,7 +1736,7 @@ class Ops:
     def _product_mxfp4(self, who: str, x: torch.Tensor | MXFP4, w: MXFP4, activation: str | None, limit: float, alpha: float,
                        out_dtype: torch.dtype, out: torch.Tensor | None) -> torch.Tensor:
         M, K, N = -1, -1, w.rows
-        both = isinstance(x, MXFP4)
+        both = type(x) is MXFP4
         if both:
             M, K, rows, ldx, x_scales, x_ld_scales = x.rows, x.cols, x.codes, x.ld_codes, x.scales.data_ptr(), x.ld_scales
         else:
@@ -1751,8 +1753,10 @@ class Ops:
                                       f"(shape {tuple(x.shape)}, strides {x.stride()})")
         if K != w.cols:
             raise KernelError(f"{who}: x is {tuple(rows.shape) if not both else (M, K)}, the weight has rows of {w.cols} numbers")
-        self._check_here(w.codes, "weight")
-        self._check_here(rows, "x")
+        here = _RAW_DEVICE() if _RAW_DEVICE is not None else torch.cuda.current_device()
+        if w.codes.get_device() != here or rows.get_device() != here:
+            self._check_here(w.codes, "weight")
+            self._check_here(rows, "x")
         cols = N if activation is None else N // 2
         if out is None:
             out = rows.new_empty((M, cols)) if rows.dtype is out_dtype else rows.new_empty((M, cols), dtype=out_dtype)
@@ -1763,16 +1767,18 @@ class Ops:
                 raise KernelError(f"{who}: out is {tuple(out.shape)}, the product {(M, cols)}")
         if M == 0 or cols == 0:
             return out
-        kind = 0 if activation is None else self.GATED_ACTIVATIONS[activation]
         scratch = None
         if not both and M <= 64:
-            size = self.lib.ts_gemm_mxfp4_scratch_bytes(M, N, K, 0)
+            size = self._scratch_mxfp4.get((M, N, K))
+            if size is None:
+                size = self._scratch_mxfp4[(M, N, K)] = int(self.lib.ts_gemm_mxfp4_scratch_bytes(M, N, K, 0))
             if size:
                 scratch = torch.empty((size,), dtype=torch.uint8, device=rows.device)
                 self.launches += 1                           # the kernel that takes x apart
+        gated, kind = (0, 0) if activation is None else (1, self.GATED_ACTIVATIONS[activation])
         self._call("ts_gemm_mxfp4", w.codes.data_ptr(), w.scales.data_ptr(), w.ld_codes, w.ld_scales, rows.data_ptr(), ldx, x_scales, x_ld_scales,
-                   out.data_ptr(), M, N, K, cols, 0 if activation is None else 1, kind, limit, alpha, 1 if w.settled else 0,
-                   _ptr(scratch), _DTYPE_CODE[out_dtype], self.error_word().data_ptr(), _stream())
+                   out.data_ptr(), M, N, K, cols, gated, kind, limit, alpha, w.settled, _ptr(scratch), _DTYPE_CODE[out_dtype],
+                   self.error_word().data_ptr(), _stream())
         return out
 
     def linear_columns(self, x: torch.Tensor, weight: torch.Tensor, out_dtype: torch.dtype | None = None) -> torch.Tensor:
