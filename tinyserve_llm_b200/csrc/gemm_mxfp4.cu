@@ -13,8 +13,13 @@ static bool few_in_registers(int M, int N, int K, bool both) {
 
 // Whether rows in bfloat16 are multiplied as two rows of 8-bit numbers each, with W's codes as they are, and not with W's codes spread to
 // bfloat16: 28,672 by 4,096 gated, 8 rows 18.4 us (spread 40.7), 64 rows 28 (42.6), 96 rows 56 (46); 2,048 by 8,192, 17 to 64 rows 10.3 to
-// 14.0 (13.9 to 15.5); 2,048 by 2,048, 64 rows 9.7 (9.0).
-static bool in_pieces(int M, int N, int K) { return K % 128 == 0 && M <= 64 && (long long)N * K > 5ll << 20; }
+// 14.0 (13.9 to 15.5); 2,048 by 2,048, 64 rows 9.7 (9.0).  More rows again where wide tiles of them fit the SMs in one round, and spreading,
+// whose tiles are smaller then, would be done over for each: 2,048 by 8,192, 512 rows 25 us (29), 1,024 rows 39 (50); 4,096 by 4,096, 384 rows
+// 22 (28); but 96 rows 23 (17).
+static bool in_pieces(int M, int N, int K) {
+    const long long numbers = (long long)N * K, wide_tiles = (long long)((N + 127) / 128) * ((2 * (long long)M + 255) / 256);
+    return K % 128 == 0 && numbers > 5ll << 20 && (M <= 64 || (M > 128 && wide_tiles <= 148));
+}
 
 // Bytes of scratch a product may need (16-byte aligned; 0: none).
 TS_API long long ts_gemm_mxfp4_scratch_bytes(int M, int N, int K, int both) {

@@ -130,7 +130,7 @@ rows16_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
     } else if (warp < 2 + EPI_WARPS) {
         // ---------------------------------------------------------------- epilogue
         const int quarter = warp & 3, first = ((warp - 2) >> 2) * SHARE;      // the 32 lanes this warp may read; its share of the columns
-        const bool paired = ((outs | (int)(p.ldy & 1)) & 1) == 0 && ((uintptr_t)p.y & 3) == 0;
+        const bool paired = (p.ldy & 1) == 0 && ((uintptr_t)p.y & 3) == 0;
         int iter = 0;
         for (int tile = first_tile; tile < num_tiles; tile += tile_step, ++iter) {
             const int buf = SPLIT ? 0 : iter & 1;

@@ -211,7 +211,7 @@ rows4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
         int iter = 0;
         for (int tile = first_tile; tile < num_tiles && ok; tile += tile_step, ++iter) {
             const int buf = SPLIT ? 0 : iter & 1;
-            ok = __all_sync(0xffffffffu, mbar_wait(&tmem_empty_bar[buf], ((iter >> 1) & 1) ^ 1, p.error, 44) && !failed);
+            ok = __all_sync(0xffffffffu, wait_for(&tmem_empty_bar[buf], ((iter >> 1) & 1) ^ 1, p.error, 44) && !failed);
             if (!ok) { failed = 1; break; }
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const uint32_t tmem_d = tmem_base + buf * BN;
@@ -246,12 +246,12 @@ rows4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
     } else if (warp < 2 + EPI_WARPS) {
         // ---------------------------------------------------------------- epilogue
         const int quarter = warp & 3, first = ((warp - 2) >> 2) * SHARE;      // the 32 lanes this warp may read; its share of the columns
-        const bool paired = ((outs | (int)(p.ldy & 1)) & 1) == 0 && ((uintptr_t)p.y & 3) == 0;
+        const bool paired = (p.ldy & 1) == 0 && ((uintptr_t)p.y & 3) == 0;
         int iter = 0;
         for (int tile = first_tile; tile < num_tiles; tile += tile_step, ++iter) {
             const int buf = SPLIT ? 0 : iter & 1;
             const int t0 = (tile % x_tiles) * (BN / PIECES), f0 = (tile / x_tiles) * OUTS;
-            const bool ok = mbar_wait(&tmem_full_bar[buf], (iter >> 1) & 1, p.error, 43) && !failed;
+            const bool ok = wait_for(&tmem_full_bar[buf], (iter >> 1) & 1, p.error, 43) && !failed;
             if (!__all_sync(0xffffffffu, ok)) { failed = 1; break; }
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             if (PIECES > 1)
@@ -426,13 +426,14 @@ template <bool GATED>
 int dispatch_pieces(const void* numbers, MxParams& p, cudaStream_t stream) {
     int sms = 148, device = 0;
     if (cudaGetDevice(&device) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
-    const int rows = p.M * PIECES8, bn = rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
+    const int rows = p.M * PIECES8, bn = rows <= 32 ? 32 : rows <= 64 ? 64 : rows <= 128 ? 128 : 256;
     const long long ldx = (long long)p.blocks * 32;
     const long long outs = GATED ? p.inter : p.N, per = GATED ? BM / 2 : BM, tiles = (outs + per - 1) / per * ((rows + bn - 1) / bn);
     p.splits = splits_of(p, tiles, sms);
     if (bn == 32) return run<8, GATED, 32, 5, true>(numbers, ldx, p, tiles, sms, device, stream);
     if (bn == 64) return run<8, GATED, 64, 4, true>(numbers, ldx, p, tiles, sms, device, stream);
-    return run<8, GATED, 128, 3, true>(numbers, ldx, p, tiles, sms, device, stream);
+    if (bn == 128) return run<8, GATED, 128, 3, true>(numbers, ldx, p, tiles, sms, device, stream);
+    return run<8, GATED, 256, 4, true>(numbers, ldx, p, tiles, sms, device, stream);
 }
 
 }  // namespace

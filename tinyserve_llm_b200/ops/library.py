@@ -1768,7 +1768,7 @@ class Ops:
         if M == 0 or cols == 0:
             return out
         scratch = None
-        if not both and M <= 64:
+        if not both:
             size = self._scratch_mxfp4.get((M, N, K))
             if size is None:
                 size = self._scratch_mxfp4[(M, N, K)] = int(self.lib.ts_gemm_mxfp4_scratch_bytes(M, N, K, 0))

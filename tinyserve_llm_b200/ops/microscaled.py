@@ -63,6 +63,6 @@ class MXFP4:
         blocks = -(-cols // BLOCK)
         ld = -(-blocks // 16) * 16
         q = cls.__new__(cls)
-        q._hold(torch.empty((rows, blocks * 16), dtype=torch.uint8, device=device),
+        q._hold(torch.empty_strided((rows, blocks * 16), (blocks * 16, 1), dtype=torch.uint8, device=device),
                 torch.empty_strided((rows, blocks), (ld, 1), dtype=torch.uint8, device=device), rows, cols, False, blocks * 16, ld)
         return q
