@@ -180,7 +180,9 @@ def test_quantize_takes_stretches_of_wider_rows(ops):
 
 # ------------------------------------------------------------------------------------------------------------ products
 SIZES = [(1, 16, 32), (1, 2048, 2048), (3, 40, 176), (7, 333, 104), (8, 512, 4096), (9, 1000, 520), (17, 130, 8), (32, 96, 8192), (33, 257, 264),
-         (64, 2048, 1024), (65, 500, 2000), (128, 129, 640), (130, 1000, 1032), (200, 70, 64), (300, 5000, 512), (700, 4100, 776), (2048, 2048, 2048)]
+         (64, 2048, 1024), (65, 500, 2000), (128, 129, 640), (130, 1000, 1032), (200, 70, 64), (300, 5000, 512), (700, 4100, 776), (2048, 2048, 2048),
+         # a few rows over larger weights, and some hundred in one round of wide tiles: rows of x in two pieces
+         (5, 9000, 2048), (9, 3001, 1792), (16, 2600, 2176), (20, 2560, 2304), (40, 2603, 2048), (64, 130, 65536), (200, 2500, 2176), (513, 700, 8192)]
 
 
 @pytest.mark.gpu
@@ -261,6 +263,34 @@ def test_what_is_not_finite_stays_in_its_row_and_column(ops, m, both):
     bad = np.zeros((m, n), dtype=bool)
     bad[1], bad[:, 7] = True, True
     np.testing.assert_array_equal(np.isnan(got), bad)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("gated", [False, True], ids=["linear", "gated"])
+@pytest.mark.parametrize("m, n, k", [(3, 300, 512), (3, 5000, 2048), (20, 5000, 1152), (20, 130, 65536), (40, 300, 512), (200, 2500, 2176), (500, 300, 512)])
+def test_infinite_numbers_in_bfloat16_rows(ops, m, n, k, gated):
+    """Infinities times numbers that are not zero are infinite, times zero or against each other NaN, beside a NaN NaN; other rows are as ever."""
+    n -= n % 2
+    x, w = numbers((m, k), torch.bfloat16, 1), f64(numbers((n, k), torch.float32, 2, 0.02))
+    x[0, 70], x[1, 5], x[1, 40], x[2, 3], x[2, 4] = float("inf"), float("inf"), float("-inf"), float("-inf"), float("nan")
+    values, xv = plain.rounded(w), f64(x)
+    with np.errstate(invalid="ignore"):
+        want, bound = xv @ values.T, sums_bound(np.where(np.isfinite(xv), xv, 0.0), values, k)
+    if gated:
+        half = n // 2
+        with np.errstate(invalid="ignore", over="ignore"):
+            g, u = want[:, :half], want[:, half:]
+            want = plain.gated("relu", g, u, 0.0, 1.0)
+            bound = bound[:, :half] * (np.abs(u) + 1) + np.abs(g) * bound[:, half:] + bound[:, :half] * bound[:, half:]
+        got = f64(ops.linear_gated_mxfp4(x.to(DEV), held(w, DEV), "relu"))
+        finite = np.isfinite(want) & np.isfinite(bound)
+        rows = slice(3, None)                                      # where gate or up is infinite, relu's NaN is the hardware's maximum
+    else:
+        got, finite, rows = f64(ops.linear_mxfp4(x.to(DEV), held(w, DEV))), np.isfinite(want), slice(None)
+        np.testing.assert_array_equal(np.isnan(got), np.isnan(want))
+        np.testing.assert_array_equal(np.where(np.isinf(got), got, 0.0), np.where(np.isinf(want), want, 0.0))
+    slack = (bound + 2.0 ** -8 * (np.abs(want) + bound))[rows][finite[rows]]
+    assert (np.abs(got - want)[rows][finite[rows]] <= slack).all()
 
 
 @pytest.mark.gpu

@@ -223,7 +223,7 @@ __device__ __forceinline__ void finish_tile(const MxParams& p, uint32_t tmem, in
 }
 
 // A split tile's share of columns, added up over the cluster's CTAs, four neighbouring lanes a thread: `id` of `threads` this one.
-// `again` works out what comes out as NaN, where that may be more than a NaN among the factors.
+// `again` gets each sum and may put another in its place.
 template <bool GATED, typename Again>
 __device__ __forceinline__ void join_splits(const MxParams& p, uint32_t sums, int rank, int columns, int t0, int f0, int outs, int id, int threads,
                                             const Again& again) {
@@ -261,15 +261,13 @@ __device__ __forceinline__ void join_splits(const MxParams& p, uint32_t sums, in
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 if (f0 + f + e >= outs) break;
-                if (v[e] != v[e]) v[e] = again(l + e, t0 + c);
-                if (u[e] != u[e]) u[e] = again(l + 16 + e, t0 + c);
-                v[e] = gate_one(p, v[e], u[e]);
+                v[e] = gate_one(p, again(l + e, t0 + c, v[e]), again(l + 16 + e, t0 + c, u[e]));
             }
         } else {
             total(c, f, v);
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-                if (f0 + f + e < outs && v[e] != v[e]) v[e] = again(f + e, t0 + c);
+                if (f0 + f + e < outs) v[e] = again(f + e, t0 + c, v[e]);
         }
 #pragma unroll
         for (int e = 0; e < 4; ++e) {

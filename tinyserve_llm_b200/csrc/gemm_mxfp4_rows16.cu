@@ -84,8 +84,10 @@ rows16_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
     // x, or the weights themselves, may come from a kernel ahead on the stream: everyone waits for those, but for the warp that brings
     // codes written long ago
     const bool codes_first = p.settled && warp == 2 + EPI_WARPS;
-    if (!codes_first) chain_wait();
-    chain_release();
+    if (!codes_first) {
+        chain_wait();
+        chain_release();
+    }
 
     if (warp == 0) {
         // ---------------------------------------------------------------- x
@@ -245,7 +247,7 @@ rows16_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
         pair_sync();                                 // every CTA's sums are in its shared memory
         const int t0 = (first_tile % x_tiles) * BN, f0 = (first_tile / x_tiles) * OUTS;
         join_splits<GATED>(p, smem_u32(stages), rank, min(BN, p.M - t0), t0, f0, outs, threadIdx.x, THREADS,
-                           [](int, int) { return __int_as_float(0x7fffffff); });
+                           [](int, int, float v) { return v; });
         __syncwarp();
         pair_sync();                                 // nobody reads another CTA's sums any more
     }

@@ -11,7 +11,8 @@
 // codes as they are; the two products are added up.  Four bits and four make a bfloat16's eight: only of numbers 2^13 times smaller than
 // their block's largest something is lost, less than 2^-21 of that largest.  An MMA of some columns costs next to nothing beside the stream of
 // W, where spreading W's codes to bfloat16, for tensor memory or in registers, takes longer than bringing them (28,672 rows of 4,096, eight
-// rows of x: 41 us).  Infinities have no place in these blocks: a result that comes out as NaN is worked out again, number by number.
+// rows of x: 41 us).  A block of x with a NaN is NaN.  Infinities have no place in these blocks: one that holds some, and no NaN, is zeros and
+// then NaN, and results whose second piece alone is NaN are worked out again, number by number.
 #include <cuda_fp16.h>
 
 #include "gemm_mxfp4.cuh"
@@ -72,6 +73,11 @@ __device__ __forceinline__ float plain_dot(const MxParams& p, int row, int t) {
     return plain_dot(p.w_codes + row * p.w_ld_codes, p.w_scales + row * p.w_ld_scales, p.x16 + t * p.x16_ld, p.K);
 }
 
+// A result from its two pieces' products; infinite (whatever its sign) stands for one that has to be worked out again.
+__device__ __forceinline__ float added(float first, float second) {
+    return second != second && first == first ? __int_as_float(0x7f800000) : first + second;
+}
+
 // The columns of a tile whose x came in two pieces a row: an epilogue warp's share, 16 columns, eight rows of x, at a time.
 template <bool GATED, int SHARE>
 __device__ __forceinline__ void finish_pieces(const MxParams& p, uint32_t tmem, int first, int t0, int f0, int outs, int quarter, int lane, float* sums) {
@@ -86,7 +92,7 @@ __device__ __forceinline__ void finish_pieces(const MxParams& p, uint32_t tmem, 
         const int column = (first + c0) / PIECES8, t = t0 + column;
         float v[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = __uint_as_float(acc[2 * j + 1]) + __uint_as_float(acc[2 * j]);
+        for (int j = 0; j < 8; ++j) v[j] = added(__uint_as_float(acc[2 * j]), __uint_as_float(acc[2 * j + 1]));
         if (p.splits > 1) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) sums[(column + j) * BM + quarter * 32 + lane] = v[j];
@@ -96,7 +102,7 @@ __device__ __forceinline__ void finish_pieces(const MxParams& p, uint32_t tmem, 
         const int row = row_of<GATED>(p, f0, quarter * 32 + lane);
 #pragma unroll
         for (int j = 0; j < 8; ++j)
-            if (v[j] != v[j] && t + j < p.M && row < p.N) v[j] = plain_dot(p, row, t + j);
+            if (isinf(v[j]) && t + j < p.M && row < p.N) v[j] = plain_dot(p, row, t + j);
         __syncwarp();
         if (GATED) {                                                  // the lower half of the lanes finishes even rows of x, the upper one odd ones
 #pragma unroll
@@ -324,7 +330,7 @@ rows4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
     if (SPLIT && p.splits > 1) {
         pair_sync();                                 // every CTA's sums are in its shared memory
         const int t0 = (first_tile % x_tiles) * (BN / PIECES), f0 = (first_tile / x_tiles) * OUTS;
-        const auto again = [&](int l, int t) { return PIECES > 1 ? plain_dot(p, min(row_of<GATED>(p, f0, l), p.N - 1), t) : __int_as_float(0x7fffffff); };
+        const auto again = [&](int l, int t, float v) { return PIECES > 1 && isinf(v) ? plain_dot(p, min(row_of<GATED>(p, f0, l), p.N - 1), t) : v; };
         join_splits<GATED>(p, smem_u32(stages), rank, min(BN / PIECES, p.M - t0), t0, f0, outs, threadIdx.x, THREADS, again);
         __syncwarp();
         pair_sync();                                 // nobody reads another CTA's sums any more
@@ -346,11 +352,11 @@ __global__ void __launch_bounds__(256) pieces_kernel(const __nv_bfloat16* __rest
                                                      uint8_t* __restrict__ scales, int M, int K, int blocks, int ld_scales) {
     chain_wait();
     chain_release();
-    const int lanes = blocks * 4, total = M * lanes;
-    const int first = blockIdx.x * 256 + (threadIdx.x & ~31), at = first + (threadIdx.x & 31);
+    const int lanes = blocks * 4;
+    const long long total = (long long)M * lanes, first = (long long)blockIdx.x * 256 + (threadIdx.x & ~31), at = first + (threadIdx.x & 31);
     if (first >= total) return;                                       // a whole warp
     const bool mine = at < total;
-    const int m = mine ? at / lanes : 0, part = mine ? at - m * lanes : 0;
+    const int m = mine ? (int)(at / lanes) : 0, part = mine ? (int)(at - (long long)m * lanes) : 0;
     float v[8];
     if (mine && part * 8 < K) {                                       // K is a multiple of 8
         const uint4 q = *reinterpret_cast<const uint4*>(x + (long long)m * ldx + part * 8);
@@ -369,7 +375,8 @@ __global__ void __launch_bounds__(256) pieces_kernel(const __nv_bfloat16* __rest
         top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
         // the largest becomes a number from 128 to 256, of 448 that there is room for
-        const int exponent = (int)(top >> 23), s = exponent == 255 ? 255 : max(exponent - 7, 0);
+        const int exponent = (int)(top >> 23);
+        int s = exponent == 255 ? 255 : max(exponent - 7, 0);
         uint2 packed = make_uint2(0, 0);
         if (exponent != 255) {
             const float inverse = __uint_as_float((uint32_t)(254 - s) << 23), scale = mx_scale(s);
@@ -387,8 +394,12 @@ __global__ void __launch_bounds__(256) pieces_kernel(const __nv_bfloat16* __rest
             }
             packed = make_uint2(two[0] | two[1] << 16, two[2] | two[3] << 16);
         } else {
+            if (i == 0 && top == 0x7f800000u) {
+                s = 0;                                                // infinities and no NaN: the second piece is NaN
+            } else {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = 0.f;                   // the first piece says NaN
+                for (int e = 0; e < 8; ++e) v[e] = 0.f;
+            }
         }
         if (mine) {
             numbers[((long long)m * PIECES8 + i) * lanes + part] = packed;
@@ -455,7 +466,7 @@ int mxfp4_pieces(const void* x, long long ldx, void* scratch, MxParams& p, int g
     p.x_ld_scales = (p.blocks + 15) / 16 * 16;
     p.x16 = (const __nv_bfloat16*)x;
     p.x16_ld = ldx;
-    TS_CHAINED_CHECK("gemm_mxfp4", launch_chained(pieces_kernel, dim3((p.M * p.blocks * 4 + 255) / 256), dim3(256), 0, stream, (const __nv_bfloat16*)x, ldx,
+    TS_CHAINED_CHECK("gemm_mxfp4", launch_chained(pieces_kernel, dim3((unsigned)(((long long)p.M * p.blocks * 4 + 255) / 256)), dim3(256), 0, stream, (const __nv_bfloat16*)x, ldx,
                                                   (uint2*)numbers, scales, p.M, p.K, p.blocks, (int)p.x_ld_scales));
     return gated ? dispatch_pieces<true>(numbers, p, stream) : dispatch_pieces<false>(numbers, p, stream);
 }

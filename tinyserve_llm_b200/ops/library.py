@@ -1771,7 +1771,9 @@ class Ops:
         if not both:
             size = self._scratch_mxfp4.get((M, N, K))
             if size is None:
-                size = self._scratch_mxfp4[(M, N, K)] = int(self.lib.ts_gemm_mxfp4_scratch_bytes(M, N, K, 0))
+                size = int(self.lib.ts_gemm_mxfp4_scratch_bytes(M, N, K, 0))
+                if M <= 64:                                  # the sizes of decode steps come again and again
+                    self._scratch_mxfp4[(M, N, K)] = size
             if size:
                 scratch = torch.empty((size,), dtype=torch.uint8, device=rows.device)
                 self.launches += 1                           # the kernel that takes x apart
