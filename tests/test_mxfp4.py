@@ -225,21 +225,20 @@ def test_gated_product(ops, m, inter, k, act, both):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("both", [False, True], ids=["rows16", "rows4"])
-@pytest.mark.parametrize("m", [2, 40, 150])
-def test_scales_from_end_to_end(ops, m, both):
+@pytest.mark.parametrize("m, n, k", [(2, 20, 320), (40, 20, 320), (150, 20, 320), (2, 5000, 1152), (40, 5000, 1152), (150, 5000, 1152)])
+def test_scales_from_end_to_end(ops, m, n, k, both):
     """Blocks under the smallest scale, scales past what one factor holds, and the largest: exact products of one column that is not zero."""
-    k, scales = 320, [0, 1, 126, 127, 128, 129, 130, 180, 251, 252]
-    w = np.zeros((20, k))
-    for i in range(20):
-        w[i, 32 * (i // 2) + 5] = (6.0 if i % 2 else -0.5) * 2.0 ** (scales[i // 2] - 127)
-    codes = np.zeros((20, 10, 32), dtype=np.uint8)
-    bytes_ = np.tile(np.array(scales, dtype=np.uint8), (20, 1))
-    for i in range(20):
-        codes[i, i // 2, 5] = 7 if i % 2 else 9
-    flat = codes.reshape(20, -1)
-    wide = torch.zeros((20, 16), dtype=torch.uint8, device=DEV)
-    wide[:, :10] = torch.from_numpy(bytes_).to(DEV)
-    weight = MXFP4(torch.from_numpy(flat[:, 0::2] | (flat[:, 1::2] << 4)).to(DEV), wide[:, :10], k)
+    scales, blocks = [0, 1, 126, 127, 128, 129, 130, 180, 251, 252], k // 32
+    w, codes, bytes_ = np.zeros((n, k)), np.zeros((n, blocks, 32), dtype=np.uint8), np.full((n, blocks), 120, dtype=np.uint8)
+    bytes_[:, :10] = scales
+    for i in range(n):
+        block, high = (i % 20) // 2, i % 2
+        w[i, 32 * block + 5] = (6.0 if high else -0.5) * 2.0 ** (scales[block] - 127)
+        codes[i, block, 5] = 7 if high else 9
+    flat = codes.reshape(n, -1)
+    wide = torch.zeros((n, -(-blocks // 16) * 16), dtype=torch.uint8, device=DEV)
+    wide[:, :blocks] = torch.from_numpy(bytes_).to(DEV)
+    weight = MXFP4(torch.from_numpy(flat[:, 0::2] | (flat[:, 1::2] << 4)).to(DEV), wide[:, :blocks], k)
     x = torch.zeros((m, k), dtype=torch.bfloat16)
     x[:, 5::32] = torch.tensor([2.0 ** (-(i % 2) - 3) for i in range(m)]).to(torch.bfloat16)[:, None]
     rows, xv = (ops.quantize_mxfp4(x.to(DEV)), plain.rounded(f64(x))) if both else (x.to(DEV), f64(x))
