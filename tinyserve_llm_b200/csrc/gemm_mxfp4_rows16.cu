@@ -8,10 +8,12 @@
 
 namespace {
 
-// Warps: producer of x, issuer, four of the epilogue, one that brings codes, teams of four that spread them: four teams, or two where tiles
-// are small and two CTAs share an SM, one's beginning and end beside the other's stream of W.
-constexpr int EPI_WARPS = 4, TEAM = 4;
-constexpr int threads_of(int teams) { return 32 * (3 + EPI_WARPS + teams * TEAM); }
+// Warps: producer of x, issuer, four of the epilogue (eight where a tile's epilogue is not under the next one's MMAs), one that brings codes,
+// teams of four that spread them: four teams, or two where tiles are small and two CTAs share an SM, one's beginning and end beside the other's
+// stream of W.
+constexpr int TEAM = 4;
+__host__ __device__ constexpr int epilogue_warps(int bn) { return bn == 256 ? 8 : 4; }
+__host__ __device__ constexpr int threads_of(int bn, int teams) { return 32 * (3 + epilogue_warps(bn) + teams * TEAM); }
 constexpr int BK = 64, PER_CHUNK = CHUNK / BK, STAGE_COLS = BK / 2;    // a stage's columns of K; of tensor memory
 
 __device__ __forceinline__ void umma(uint32_t leader, uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
@@ -31,11 +33,12 @@ __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&r)[16]
 
 // BN: rows of x a tile.  STAGES: x's ring.  PACKED: chunks of codes in shared memory.  MADE: stages of numbers in tensor memory.
 template <bool GATED, int BN, int STAGES, int PACKED, bool SPLIT, int TEAMS>
-__global__ void __launch_bounds__(32 * (3 + EPI_WARPS + TEAMS * TEAM), TEAMS == 2 ? 2 : 1)
+__global__ void __launch_bounds__(threads_of(BN, TEAMS), TEAMS == 2 ? 2 : 1)
 rows16_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, MxParams p) {
-    constexpr int B_BYTES = BN * ROW, ACCUMULATORS = SPLIT ? 1 : 2, OUTS = GATED ? BM / 2 : BM, SHARE = BN / (EPI_WARPS / 4);
-    constexpr int THREADS = 32 * (3 + EPI_WARPS + TEAMS * TEAM);
-    constexpr int MADE = STAGES < 8 || TEAMS == 2 || (512 - ACCUMULATORS * BN) / STAGE_COLS < 8 ? 4 : 8, TMEM_COLS = power_of_two(ACCUMULATORS * BN + MADE * STAGE_COLS);
+    constexpr int EPI_WARPS = epilogue_warps(BN), THREADS = threads_of(BN, TEAMS);
+    constexpr int B_BYTES = BN * ROW, ACCUMULATORS = SPLIT || BN == 256 ? 1 : 2, OUTS = GATED ? BM / 2 : BM, SHARE = BN / (EPI_WARPS / 4);
+    constexpr int ROOM = (512 - ACCUMULATORS * BN) / STAGE_COLS, MADE = TEAMS == 2 ? 4 : STAGES < 8 ? (STAGES < ROOM ? STAGES : ROOM) : ROOM < 8 ? 4 : 8;
+    constexpr int TMEM_COLS = power_of_two(ACCUMULATORS * BN + MADE * STAGE_COLS);
     static_assert(TMEM_COLS * (TEAMS == 2 ? 2 : 1) <= 512 && ACCUMULATORS * BN + MADE * STAGE_COLS <= TMEM_COLS, "tensor memory has 512 columns");
     static_assert(STAGES >= MADE, "a stage's barriers go round once more only after its place in tensor memory has been waited for");
     static_assert(!SPLIT || BM * BN * 4 <= STAGES * B_BYTES, "a split tile's sums go where the ring was");
@@ -111,8 +114,8 @@ rows16_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
         const uint64_t b_first = smem_desc(stages);
         int iter = 0;
         for (int tile = first_tile; tile < num_tiles && ok; tile += tile_step, ++iter) {
-            const int buf = SPLIT ? 0 : iter & 1;
-            ok = __all_sync(0xffffffffu, mbar_wait(&tmem_empty_bar[buf], ((iter >> 1) & 1) ^ 1, p.error, 44) && !failed);
+            const int buf = ACCUMULATORS == 1 ? 0 : iter & 1, round = ACCUMULATORS == 1 ? iter : iter >> 1;
+            ok = __all_sync(0xffffffffu, mbar_wait(&tmem_empty_bar[buf], (round & 1) ^ 1, p.error, 44) && !failed);
             if (!ok) { failed = 1; break; }
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const uint32_t tmem_d = tmem_base + buf * BN;
@@ -135,9 +138,9 @@ rows16_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
         const bool paired = (p.ldy & 1) == 0 && ((uintptr_t)p.y & 3) == 0;
         int iter = 0;
         for (int tile = first_tile; tile < num_tiles; tile += tile_step, ++iter) {
-            const int buf = SPLIT ? 0 : iter & 1;
+            const int buf = ACCUMULATORS == 1 ? 0 : iter & 1, round = ACCUMULATORS == 1 ? iter : iter >> 1;
             const int t0 = (tile % x_tiles) * BN, f0 = (tile / x_tiles) * OUTS;
-            const bool ok = mbar_wait(&tmem_full_bar[buf], (iter >> 1) & 1, p.error, 43) && !failed;
+            const bool ok = mbar_wait(&tmem_full_bar[buf], round & 1, p.error, 43) && !failed;
             if (!__all_sync(0xffffffffu, ok)) { failed = 1; break; }
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             finish_tile<GATED, SHARE, SPLIT>(p, tmem_base + buf * BN, first, t0, f0, outs, paired, quarter, lane, reinterpret_cast<float*>(stages),
@@ -269,7 +272,7 @@ int run(const void* x, long long ldx, MxParams& p, long long tiles, int sms, int
     if (make_codes_map<GATED>(&map_w, p)) return 1;
     if (make_tile_map(&map_x, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, x, p.M, p.K, ldx, BN, "gemm_mxfp4")) return 1;
     static unsigned long long allowed = 0;
-    return launch_mxfp4(rows16_kernel<GATED, BN, STAGES, PACKED, SPLIT, TEAMS>, allowed, threads_of(TEAMS),
+    return launch_mxfp4(rows16_kernel<GATED, BN, STAGES, PACKED, SPLIT, TEAMS>, allowed, threads_of(BN, TEAMS),
                         (size_t)STAGES * BN * ROW + PACKED * A_BYTES + 1024, SPLIT, tiles, sms, device, map_w, map_x, p, stream);
 }
 
@@ -277,9 +280,8 @@ template <bool GATED>
 int dispatch(const void* x, long long ldx, MxParams& p, cudaStream_t stream) {
     int sms = 148, device = 0;
     if (cudaGetDevice(&device) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
-    return cut_mxfp4<GATED, 192>(p, p.M, sms, [&](int bn, bool split, long long tiles) {
-        if (bn == 256) return run<GATED, 256, 5, 3, true, 4>(x, ldx, p, tiles, sms, device, stream);
-        if (bn == 192) return run<GATED, 192, 6, 4, false, 4>(x, ldx, p, tiles, sms, device, stream);
+    return cut_mxfp4<GATED, 256>(p, p.M, sms, [&](int bn, bool split, long long tiles) {
+        if (bn == 256) return run<GATED, 256, 5, 3, false, 4>(x, ldx, p, tiles, sms, device, stream);
         if (bn == 128) return split ? run<GATED, 128, 4, 2, true, 2>(x, ldx, p, tiles, sms, device, stream)
                                     : run<GATED, 128, 8, 4, false, 4>(x, ldx, p, tiles, sms, device, stream);
         if (bn == 64) return run<GATED, 64, 6, 3, true, 2>(x, ldx, p, tiles, sms, device, stream);
