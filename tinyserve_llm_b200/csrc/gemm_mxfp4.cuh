@@ -7,8 +7,8 @@
 // Gated (y = act(x Wgate^T, x Wup^T), W = [gate rows | up rows]): a tile holds 16 gate rows, the 16 up rows that belong to them, and so
 // on, so that a gate lies 16 lanes before its up in the same warp's quarter of tensor memory and one shuffle brings them together.
 //
-// Many tiles: persistent, one CTA an SM, two accumulators, so that a tile's epilogue runs under the next one's MMAs.  Few tiles: a cluster
-// of `splits` CTAs takes a tile, each its share of K, and leaves its sums in its own shared memory; each CTA then adds up a share of the
+// Many tiles: persistent, one CTA an SM, with two accumulators, so that a tile's epilogue runs under the next one's MMAs, or one of 256 columns,
+// beside whose epilogue the next tile's operands are made.  Few tiles: a cluster of `splits` CTAs takes a tile, each its share of K, and leaves its sums in its own shared memory; each CTA then adds up a share of the
 // columns from all of them, in the order of their ranks.  Nothing of that needs a workspace in global memory, and the order is fixed.
 //
 // Every wait on an mbarrier gives up after about two seconds, records where in an error word the host can read, and the CTA goes on to
@@ -82,6 +82,13 @@ __device__ __forceinline__ void tmem_ld16(uint32_t addr, uint32_t (&r)[16]) {
         : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
           "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
         : "r"(addr) : "memory");
+}
+
+// What tmem_ld16 reads is there; named, so that nothing that uses it comes before.
+__device__ __forceinline__ void tmem_wait16(uint32_t (&r)[16]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]),
+                   "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])::"memory");
 }
 
 // The activation is chosen once for many values, so that what runs is one short loop and not four activations in a row.
@@ -207,7 +214,7 @@ __device__ __forceinline__ void finish_tile(const MxParams& p, uint32_t tmem, in
         uint32_t acc[16];
         __syncwarp();
         tmem_ld16(addr + c0, acc);
-        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+        tmem_wait16(acc);
         if (!SPLIT && c0 + 16 == SHARE) {                             // the last of it: the accumulator goes back before the stores
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             __syncwarp();

@@ -3,7 +3,12 @@
 // W's codes come into shared memory by TMA as they are, 128 rows of a chunk at a time; sixteen warps make bfloat16 numbers of them (exactly)
 // and store them into tensor memory, where tcgen05.mma kind::f16 takes its first operand from; x comes by TMA, 64 numbers a row and stage, and
 // is the second.  Shared memory's 128 bytes a cycle would bound the other way: with the numbers laid there too, 16 KB more are written and read
-// per 64 columns of K, beside 32 KB of x written and read, against 512 cycles of MMAs of 256 columns (2,048 rows, 8,192 by 2,048: 58 us).
+// per 64 columns of K, beside 32 KB of x written and read, against 512 cycles of MMAs of 256 columns (2,048 rows, 8,192 by 2,048: 58 us; 49 now).
+//
+// Bound by instructions: some 1,900 of a warp for 64 columns of K and a tile, half of them the codes' (27 for a warp's 8 x 32 codes), at 0.64 of the
+// issue slots, tensor cores 0.67 busy.  So tiles are as wide as tensor memory lets them be: 256 rows of x on one accumulator, spread codes serve 256 columns, and a tile's
+// epilogue costs less than it would save to hide it: gated 2,048 rows over 2 x 8,192 by 2,048 115 us with 192 rows and two accumulators, 106 with
+// 256 and one (1.30 PFLOP/s); 2,048 rows through an 8B model's gate and up projections 376 and 344 (1.40).
 #include "gemm_mxfp4.cuh"
 
 namespace {

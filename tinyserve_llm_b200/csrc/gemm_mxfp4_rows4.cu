@@ -88,7 +88,7 @@ __device__ __forceinline__ void finish_pieces(const MxParams& p, uint32_t tmem, 
         uint32_t acc[16];
         __syncwarp();
         tmem_ld16(addr + c0, acc);
-        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+        tmem_wait16(acc);
         const int column = (first + c0) / PIECES8, t = t0 + column;
         float v[8];
 #pragma unroll
