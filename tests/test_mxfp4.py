@@ -266,7 +266,8 @@ def test_what_is_not_finite_stays_in_its_row_and_column(ops, m, both):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("gated", [False, True], ids=["linear", "gated"])
-@pytest.mark.parametrize("m, n, k", [(3, 300, 512), (3, 5000, 2048), (20, 5000, 1152), (20, 130, 65536), (40, 300, 512), (200, 2500, 2176), (500, 300, 512)])
+@pytest.mark.parametrize("m, n, k", [(3, 300, 512), (3, 5000, 2048), (20, 5000, 1152), (20, 130, 65536), (40, 300, 512), (200, 2500, 2176),
+                                     (500, 300, 512)])
 def test_infinite_numbers_in_bfloat16_rows(ops, m, n, k, gated):
     """Infinities times numbers that are not zero are infinite, times zero or against each other NaN, beside a NaN NaN; other rows are as ever."""
     n -= n % 2

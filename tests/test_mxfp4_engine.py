@@ -123,6 +123,18 @@ def test_a_model_without_such_parts_is_refused(tmp_path):
 
 
 @pytest.mark.gpu
+def test_trace_replay_takes_the_formats(model_folders, tmp_path):
+    proc = subprocess.run(
+        [sys.executable, ru.TRACE_RUN, "--model", model_folders["a"], "--dtype", "bfloat16", "--out", str(tmp_path), "--max-tokens", "128",
+         "--weight-format", "mxfp4", "--activation-format", "mxfp4"],
+        input=json.dumps({"step": 0, "entries": [{"id": "a", "tokens": [5, 17, 3], "want": [2]}], "end": ["a"]}) + "\n",
+        capture_output=True, text=True, timeout=600)
+    assert proc.returncode == 0 and proc.stdout.split() == ["done", "0"], proc.stderr[-3000:]
+    calls = json.loads((tmp_path / "stats.json").read_text())["kernel_calls"]
+    assert calls["ts_gemm_mxfp4"] == 4 * TINY_A["num_hidden_layers"] and calls["ts_quantize_mxfp4"] == 2 * calls["ts_gemm_mxfp4"]
+
+
+@pytest.mark.gpu
 def test_generate_and_the_command_line(model_folders, tmp_path):
     from tinyserve_llm_b200 import LLM, CacheConfig, SamplingParams, SchedulerConfig
     folder, prompts = model_folders["a"], [[1, 2, 3, 4], [9, 8, 7]]

@@ -29,7 +29,8 @@ TS_API long long ts_gemm_mxfp4_scratch_bytes(int M, int N, int K, int both) {
 
 // y = x . W^T (gated 0; y [M, N], bfloat16 or float32) or y = act(x Wgate^T, x Wup^T) with W = [gate rows | up rows] (gated 1; y [M, N / 2],
 // bfloat16; TS_ACT_* of common.cuh).  x: bfloat16 [M, K], rows ldx elements apart, if x_scales is null; else codes, rows ldx bytes apart,
-// and scales.  settled: nothing that may still run ahead on the stream writes W.  K a multiple of 8 (rows in bfloat16); rows of codes and of scales start 16-byte aligned, and so do x and its rows.
+// and scales.  settled: nothing that may still run ahead on the stream writes W.  K a multiple of 8 (rows in bfloat16); rows of codes and of
+// scales start 16-byte aligned, and so do x and its rows.
 TS_API int ts_gemm_mxfp4(const void* w_codes, const void* w_scales, long long w_ld_codes, long long w_ld_scales, const void* x, long long ldx,
                          const void* x_scales, long long x_ld_scales, void* y, int M, int N, int K, long long ldy, int gated, int act,
                          float limit, float alpha, int settled, void* scratch, int out_dtype, int* error, cudaStream_t stream) {

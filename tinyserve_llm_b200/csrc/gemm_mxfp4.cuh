@@ -8,8 +8,8 @@
 // on, so that a gate lies 16 lanes before its up in the same warp's quarter of tensor memory and one shuffle brings them together.
 //
 // Many tiles: persistent, one CTA an SM, with two accumulators, so that a tile's epilogue runs under the next one's MMAs, or one of 256 columns,
-// beside whose epilogue the next tile's operands are made.  Few tiles: a cluster of `splits` CTAs takes a tile, each its share of K, and leaves its sums in its own shared memory; each CTA then adds up a share of the
-// columns from all of them, in the order of their ranks.  Nothing of that needs a workspace in global memory, and the order is fixed.
+// beside whose epilogue the next tile's operands are made.  Few tiles: a cluster of `splits` CTAs takes a tile, each its share of K, and leaves
+// its sums in its own shared memory; each CTA then adds up a share of the columns from all of them, in the order of their ranks.  Nothing of that needs a workspace in global memory, and the order is fixed.
 //
 // Every wait on an mbarrier gives up after about two seconds, records where in an error word the host can read, and the CTA goes on to
 // free its tensor memory and return.
@@ -203,7 +203,8 @@ int make_codes_map(CUtensorMap* map, MxParams& p, bool spaced = false) {
     return 0;
 }
 
-// An epilogue warp's share of a tile: columns `first` to `first + SHARE` of the accumulator at `tmem`.  `sums`: where a split tile's go, [column][lane].
+// An epilogue warp's share of a tile: columns `first` to `first + SHARE` of the accumulator at `tmem`.  `sums`: where a split tile's go, by column
+// and lane.
 template <bool GATED, int SHARE, bool SPLIT>
 __device__ __forceinline__ void finish_tile(const MxParams& p, uint32_t tmem, int first, int t0, int f0, int outs, bool paired, int quarter, int lane,
                                             float* sums, uint64_t* drained) {

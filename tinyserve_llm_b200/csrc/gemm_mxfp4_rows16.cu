@@ -6,8 +6,8 @@
 // per 64 columns of K, beside 32 KB of x written and read, against 512 cycles of MMAs of 256 columns (2,048 rows, 8,192 by 2,048: 58 us; 49 now).
 //
 // Bound by instructions: some 1,900 of a warp for 64 columns of K and a tile, half of them the codes' (27 for a warp's 8 x 32 codes), at 0.64 of the
-// issue slots, tensor cores 0.67 busy.  So tiles are as wide as tensor memory lets them be: 256 rows of x on one accumulator, spread codes serve 256 columns, and a tile's
-// epilogue costs less than it would save to hide it: gated 2,048 rows over 2 x 8,192 by 2,048 115 us with 192 rows and two accumulators, 106 with
+// issue slots, tensor cores 0.67 busy.  So tiles are as wide as tensor memory lets them be, 256 rows of x on one accumulator: codes once spread
+// serve 256 columns, and a tile's epilogue costs less than it would save to hide it.  Gated 2,048 rows over 2 x 8,192 by 2,048 115 us with 192 rows and two accumulators, 106 with
 // 256 and one (1.30 PFLOP/s); 2,048 rows through an 8B model's gate and up projections 376 and 344 (1.40).
 #include "gemm_mxfp4.cuh"
 
@@ -42,13 +42,15 @@ __global__ void __launch_bounds__(threads_of(BN, TEAMS), TEAMS == 2 ? 2 : 1)
 rows16_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, MxParams p) {
     constexpr int EPI_WARPS = epilogue_warps(BN), THREADS = threads_of(BN, TEAMS);
     constexpr int B_BYTES = BN * ROW, ACCUMULATORS = SPLIT || BN == 256 ? 1 : 2, OUTS = GATED ? BM / 2 : BM, SHARE = BN / (EPI_WARPS / 4);
-    constexpr int ROOM = (512 - ACCUMULATORS * BN) / STAGE_COLS, MADE = TEAMS == 2 ? 4 : STAGES < 8 ? (STAGES < ROOM ? STAGES : ROOM) : ROOM < 8 ? 4 : 8;
+    constexpr int ROOM = (512 - ACCUMULATORS * BN) / STAGE_COLS;
+    constexpr int MADE = TEAMS == 2 ? 4 : STAGES < 8 ? (STAGES < ROOM ? STAGES : ROOM) : ROOM < 8 ? 4 : 8;
     constexpr int TMEM_COLS = power_of_two(ACCUMULATORS * BN + MADE * STAGE_COLS);
     static_assert(TMEM_COLS * (TEAMS == 2 ? 2 : 1) <= 512 && ACCUMULATORS * BN + MADE * STAGE_COLS <= TMEM_COLS, "tensor memory has 512 columns");
     static_assert(STAGES >= MADE, "a stage's barriers go round once more only after its place in tensor memory has been waited for");
     static_assert(!SPLIT || BM * BN * 4 <= STAGES * B_BYTES, "a split tile's sums go where the ring was");
     extern __shared__ __align__(1024) unsigned char smem_raw[];
-    __shared__ __align__(8) uint64_t full_bar[STAGES], empty_bar[STAGES], tmem_full_bar[2], tmem_empty_bar[2], packed_full[PACKED], packed_empty[PACKED];
+    __shared__ __align__(8) uint64_t full_bar[STAGES], empty_bar[STAGES], tmem_full_bar[2], tmem_empty_bar[2];
+    __shared__ __align__(8) uint64_t packed_full[PACKED], packed_empty[PACKED];
     __shared__ uint32_t tmem_base_slot;
     __shared__ int failed;
 
@@ -169,8 +171,8 @@ rows16_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
     } else {
         // ---------------------------------------------------------------- codes to bfloat16 numbers
         // Team j makes quarter j of every chunk (of two teams each makes two), one stage, so that as many stages are in the making at a time; a
-        // thread takes the row of its lane of tensor memory and both blocks of its quarter.  Eight lanes that read shared memory together have eight neighbouring rows, whose
-        // 16-byte pieces the swizzle puts into different banks.
+        // thread takes the row of its lane of tensor memory and both blocks of its quarter.  Eight lanes that read shared memory together have
+        // eight neighbouring rows, whose 16-byte pieces the swizzle puts into different banks.
         const int team = (warp - 3 - EPI_WARPS) / TEAM, l = (warp & 3) * 32 + lane;
         const uint32_t to = tmem_made + ((uint32_t)((warp & 3) * 32) << 16);
         bool ok = true;

@@ -80,7 +80,8 @@ __device__ __forceinline__ float added(float first, float second) {
 
 // The columns of a tile whose x came in two pieces a row: an epilogue warp's share, 16 columns, eight rows of x, at a time.
 template <bool GATED, int SHARE>
-__device__ __forceinline__ void finish_pieces(const MxParams& p, uint32_t tmem, int first, int t0, int f0, int outs, int quarter, int lane, float* sums) {
+__device__ __forceinline__ void finish_pieces(const MxParams& p, uint32_t tmem, int first, int t0, int f0, int outs, int quarter, int lane,
+                                              float* sums) {
     const uint32_t addr = tmem + first + ((uint32_t)(quarter * 32) << 16);
     const int f = GATED ? f0 + quarter * 16 + (lane & 15) : f0 + quarter * 32 + lane;
 #pragma unroll 1
@@ -147,7 +148,8 @@ rows4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
     static_assert(PIECES == 1 || SPLIT, "pieces are added up by tiles");
     static_assert(!SPLIT || BM * BN / PIECES * 4 <= STAGES * (A_BYTES + B_BYTES), "a split tile's sums go where the ring was");
     extern __shared__ __align__(1024) unsigned char smem_raw[];
-    __shared__ __align__(8) uint64_t full_bar[STAGES], empty_bar[STAGES], tmem_full_bar[2], tmem_empty_bar[2], scales_full[GROUPS_HELD], scales_empty[GROUPS_HELD];
+    __shared__ __align__(8) uint64_t full_bar[STAGES], empty_bar[STAGES], tmem_full_bar[2], tmem_empty_bar[2];
+    __shared__ __align__(8) uint64_t scales_full[GROUPS_HELD], scales_empty[GROUPS_HELD];
     __shared__ uint32_t tmem_base_slot;
     __shared__ int failed;
 
@@ -200,7 +202,7 @@ rows4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
                     const int s = r.at;
                     if (!wait_for(&empty_bar[s], r.parity ^ 1, p.error, 41)) { failed = 1; break; }
                     unsigned char* tile_at = stages + s * (A_BYTES + B_BYTES);
-                    mbar_expect_tx(&full_bar[s], (KIND == 4 ? A_BYTES : A_BYTES / 2) + B_BYTES);      // codes that are spaced out count without the space
+                    mbar_expect_tx(&full_bar[s], (KIND == 4 ? A_BYTES : A_BYTES / 2) + B_BYTES);      // spaced codes count without the space
                     load_codes<GATED>(tile_at, &map_w, &full_bar[s], p, chunk * ROW, f0);
                     tma_load_2d(tile_at + A_BYTES, &map_x, &full_bar[s], chunk * ROW, t0 * PIECES);
                 }
@@ -224,7 +226,8 @@ rows4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
             uint32_t add = 0;                        // the tile's first MMA starts its sums
             for (int chunk = chunk0; chunk < chunk1; ++chunk, r.next()) {
                 ok = __all_sync(0xffffffffu, wait_for(&full_bar[r.at], r.parity, p.error, 42));
-                if (chunk == chunk0 || (chunk & (PER_GROUP - 1)) == 0) ok = __all_sync(0xffffffffu, ok && wait_for(&scales_full[g.at], g.parity, p.error, 49));
+                if (chunk == chunk0 || (chunk & (PER_GROUP - 1)) == 0)
+                    ok = __all_sync(0xffffffffu, ok && wait_for(&scales_full[g.at], g.parity, p.error, 49));
                 if (!ok) { failed = 1; break; }
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const uint64_t a_desc = a_first + r.at * ((A_BYTES + B_BYTES) / 16), b_desc = b_first + r.at * ((A_BYTES + B_BYTES) / 16);
@@ -311,7 +314,8 @@ rows4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
                     const int g = w + i * GATHER;
                     if (g >= GROUPS) continue;
                     // word j of the row: stage j / SETS of the group, set j % SETS
-                    unsigned char* to = scale_ring + r.at * PER_GROUP * SCALE_BYTES + lane * 16 + (g & 3) * 4 + (g < 4 ? 0 : SETS * 512 + ((g - 4) >> 2) * 512);
+                    const int of_x = g < 4 ? 0 : SETS * 512 + ((g - 4) >> 2) * 512;
+                    unsigned char* to = scale_ring + r.at * PER_GROUP * SCALE_BYTES + of_x + lane * 16 + (g & 3) * 4;
                     const int set = g < 4 ? 512 : X_SETS * 512;
                     *reinterpret_cast<uint32_t*>(to) = now[i].x;
                     *reinterpret_cast<uint32_t*>(to + (SETS == 2 ? set : SCALE_BYTES)) = now[i].y;
@@ -466,7 +470,8 @@ int mxfp4_pieces(const void* x, long long ldx, void* scratch, MxParams& p, int g
     p.x_ld_scales = (p.blocks + 15) / 16 * 16;
     p.x16 = (const __nv_bfloat16*)x;
     p.x16_ld = ldx;
-    TS_CHAINED_CHECK("gemm_mxfp4", launch_chained(pieces_kernel, dim3((unsigned)(((long long)p.M * p.blocks * 4 + 255) / 256)), dim3(256), 0, stream, (const __nv_bfloat16*)x, ldx,
-                                                  (uint2*)numbers, scales, p.M, p.K, p.blocks, (int)p.x_ld_scales));
+    const dim3 grid((unsigned)(((long long)p.M * p.blocks * 4 + 255) / 256));
+    TS_CHAINED_CHECK("gemm_mxfp4", launch_chained(pieces_kernel, grid, dim3(256), 0, stream, (const __nv_bfloat16*)x, ldx, (uint2*)numbers, scales,
+                                                  p.M, p.K, p.blocks, (int)p.x_ld_scales));
     return gated ? dispatch_pieces<true>(numbers, p, stream) : dispatch_pieces<false>(numbers, p, stream);
 }
