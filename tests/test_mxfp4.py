@@ -77,6 +77,25 @@ def test_container_refuses_what_the_kernels_do_not_take():
     assert MXFP4(wide[:, 16:64], q.scales, 70).ld_codes == 64
 
 
+def test_sizes_past_the_kernels_whole_numbers_are_refused():
+    """The kernels count rows and columns in 32 bits: what they would count wrongly (4,294,967,328 columns as 32) never reaches them."""
+    from tinyserve_llm_b200.ops import Ops
+    ops, bare = Ops.__new__(Ops), lambda shape, dtype: torch.empty(shape, dtype=dtype, device="meta")
+    for cols in (2 ** 30, 2 ** 31 + 32, 2 ** 32 + 32):
+        with pytest.raises(KernelError, match="columns"):
+            ops.quantize_mxfp4(bare((1, cols), torch.bfloat16))
+        with pytest.raises(ValueError, match="numbers"):
+            MXFP4(bare((1, cols // 2), torch.uint8), bare((1, cols // 32), torch.uint8), cols)
+    tall = lambda rows: MXFP4(bare((rows, 16), torch.uint8), bare((rows, 16), torch.uint8)[:, :1], 32)  # noqa: E731
+    for rows in (2 ** 30, 2 ** 32 + 6):
+        with pytest.raises(KernelError, match="rows"):
+            ops.linear_mxfp4(bare((rows, 32), torch.bfloat16), tall(6))
+        with pytest.raises(KernelError, match="rows"):
+            ops.linear_mxfp4(bare((4, 32), torch.bfloat16), tall(rows))
+        with pytest.raises(KernelError, match="rows"):
+            ops.linear_gated_mxfp4(tall(rows), tall(6), "silu")
+
+
 def test_oracle_rounds_to_the_nearest_of_two():
     x = np.array([[0.0, -0.0, 0.25, 0.2500001, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, 5.0001, 6.0, 7.0, 7.9, -0.75, -3.5] + [0.0] * 16])
     want = [0, 0, 0, 0.5, 1, 1, 2, 2, 4, 4, 6, 6, 6, 6, -1, -4]
@@ -290,7 +309,38 @@ def test_infinite_numbers_in_bfloat16_rows(ops, m, n, k, gated):
         np.testing.assert_array_equal(np.isnan(got), np.isnan(want))
         np.testing.assert_array_equal(np.where(np.isinf(got), got, 0.0), np.where(np.isinf(want), want, 0.0))
     slack = (bound + 2.0 ** -8 * (np.abs(want) + bound))[rows][finite[rows]]
-    assert (np.abs(got - want)[rows][finite[rows]] <= slack).all()
+    with np.errstate(invalid="ignore"):
+        assert (np.abs(got - want)[rows][finite[rows]] <= slack).all()
+
+
+@pytest.mark.gpu
+def test_offsets_past_32_bits(ops):
+    """Two thousand million outputs and more: the last rows are what a product of theirs alone gives, and so are the last rows' codes."""
+    m, n, k = 20032, 110080, 64
+    w, x = held(f64(numbers((n, k), torch.float32, 21, 0.05)), DEV), numbers((m, k), torch.bfloat16, 22).to(DEV)
+    values = f64(ops.dequantize_mxfp4(w, torch.float32))
+    for rows, xv in ((x, f64(x[-40:])), (ops.quantize_mxfp4(x), plain.rounded(f64(x[-40:])))):
+        y = ops.linear_mxfp4(rows, w)
+        assert y.numel() > 2 ** 31
+        check(y[-40:], xv @ values.T, sums_bound(xv, values, k))
+    q = ops.quantize_mxfp4(y.t().contiguous())
+    tail = ops.quantize_mxfp4(y[:, -3:].t().contiguous())
+    assert torch.equal(q.codes[-3:], tail.codes) and torch.equal(q.scales[-3:], tail.scales)
+    assert torch.equal(ops.dequantize_mxfp4(q)[-3:], ops.dequantize_mxfp4(tail))
+    ops.check_device_errors()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("both", [False, True], ids=["rows16", "rows4"])
+@pytest.mark.parametrize("m, n, k", [(4, 256, 512), (40, 5120, 1152), (200, 512, 256), (400, 2048, 4096)])
+def test_out_that_starts_between_words(ops, m, n, k, both):
+    w, x = held(f64(numbers((n, k), torch.float32, 23, 0.02)), DEV), numbers((m, k), torch.bfloat16, 24).to(DEV)
+    x = ops.quantize_mxfp4(x) if both else x
+    room = torch.full((m * n + 2,), 7.0, dtype=torch.bfloat16, device=DEV)
+    out = room[1:-1].view(m, n)
+    assert out.data_ptr() % 4 == 2
+    assert torch.equal(ops.linear_mxfp4(x, w, out=out), ops.linear_mxfp4(x, w))
+    assert float(room[0]) == 7 and float(room[-1]) == 7
 
 
 @pytest.mark.gpu

@@ -34,7 +34,7 @@ TS_API long long ts_gemm_mxfp4_scratch_bytes(int M, int N, int K, int both) {
 TS_API int ts_gemm_mxfp4(const void* w_codes, const void* w_scales, long long w_ld_codes, long long w_ld_scales, const void* x, long long ldx,
                          const void* x_scales, long long x_ld_scales, void* y, int M, int N, int K, long long ldy, int gated, int act,
                          float limit, float alpha, int settled, void* scratch, int out_dtype, int* error, cudaStream_t stream) {
-    TS_REQUIRE(M >= 0 && N > 0 && K > 0 && K <= 0x3fffffff, "gemm_mxfp4: bad sizes M=%d N=%d K=%d", M, N, K);
+    TS_REQUIRE(M >= 0 && M <= MX_MOST && N > 0 && N <= MX_MOST && K > 0 && K <= MX_MOST, "gemm_mxfp4: bad sizes M=%d N=%d K=%d", M, N, K);
     TS_REQUIRE(out_dtype == TS_BF16 || (out_dtype == TS_F32 && !gated), "gemm_mxfp4: unsupported output dtype %d", out_dtype);
     TS_REQUIRE(!gated || (N % 2 == 0 && act >= TS_ACT_SILU && act <= TS_ACT_LAST), "gemm_mxfp4: N=%d, activation %d", N, act);
     TS_REQUIRE(x_scales || K % 8 == 0, "gemm_mxfp4: K=%d is not a multiple of 8", K);

@@ -139,7 +139,7 @@ __global__ void __launch_bounds__(THREADS) dequantize_mxfp4_kernel(const uint2* 
 // codes: rows of 16 bytes a block; scales: rows of one byte a block, ld_scales apart.
 TS_API int ts_quantize_mxfp4(const void* x, void* codes, void* scales, long long rows, int cols, long long ldx, long long ld_codes,
                              long long ld_scales, int dtype, cudaStream_t stream) {
-    TS_REQUIRE(rows >= 0 && cols > 0, "quantize_mxfp4: bad sizes: %lld rows of %d", rows, cols);
+    TS_REQUIRE(rows >= 0 && cols > 0 && cols <= MX_MOST, "quantize_mxfp4: bad sizes: %lld rows of %d", rows, cols);
     TS_REQUIRE(dtype == TS_F32 || dtype == TS_BF16, "quantize_mxfp4: unknown dtype %d", dtype);
     const int blocks = (cols + MX_BLOCK - 1) / MX_BLOCK, size = dtype == TS_F32 ? 4 : 2;
     TS_REQUIRE(ld_codes >= (long long)blocks * 16 && ld_codes % 8 == 0 && (uintptr_t)codes % 8 == 0 && ld_scales >= blocks,
@@ -160,7 +160,7 @@ TS_API int ts_quantize_mxfp4(const void* x, void* codes, void* scales, long long
 
 TS_API int ts_dequantize_mxfp4(const void* codes, const void* scales, void* y, long long rows, int cols, long long ld_codes,
                                long long ld_scales, int dtype, cudaStream_t stream) {
-    TS_REQUIRE(rows >= 0 && cols > 0, "dequantize_mxfp4: bad sizes: %lld rows of %d", rows, cols);
+    TS_REQUIRE(rows >= 0 && cols > 0 && cols <= MX_MOST, "dequantize_mxfp4: bad sizes: %lld rows of %d", rows, cols);
     TS_REQUIRE(dtype == TS_F32 || dtype == TS_BF16, "dequantize_mxfp4: unknown dtype %d", dtype);
     const int blocks = (cols + MX_BLOCK - 1) / MX_BLOCK, size = dtype == TS_F32 ? 4 : 2;
     TS_REQUIRE(ld_codes >= (long long)blocks * 16 && ld_codes % 8 == 0 && (uintptr_t)codes % 8 == 0 && ld_scales >= blocks,

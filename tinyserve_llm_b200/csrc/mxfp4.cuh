@@ -7,6 +7,7 @@
 #include "common.cuh"
 
 constexpr int MX_BLOCK = 32;
+constexpr int MX_MOST = 0x3fffffff;              // columns of a matrix, rows of a product: counted in 32 bits, with room for a block or a doubling
 
 // 2^(s - 127) as float32; NaN for s = 255.
 __device__ __forceinline__ float mx_scale(uint32_t s) {

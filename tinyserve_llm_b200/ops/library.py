@@ -13,7 +13,7 @@ import os
 import torch
 
 from tinyserve_llm_b200.ops.build import build_library
-from tinyserve_llm_b200.ops.microscaled import MXFP4
+from tinyserve_llm_b200.ops.microscaled import MOST, MXFP4
 
 _DTYPE_CODE = {torch.float32: 0, torch.bfloat16: 1}
 
@@ -1689,8 +1689,8 @@ class Ops:
         if x.dim() != 2 or x.dtype not in _DTYPE_CODE or (x.shape[1] > 1 and x.stride(1) != 1):
             raise KernelError(f"quantize_mxfp4: x must be a [rows, columns] stretch of float32 or bfloat16, got {x.dtype} {tuple(x.shape)}")
         rows, cols = x.shape
-        if cols == 0:
-            raise KernelError("quantize_mxfp4: x has no columns")
+        if not 0 < cols <= MOST:
+            raise KernelError(f"quantize_mxfp4: x has {cols} columns; 1 to {MOST} can be held")
         self._check_here(x, "x")
         q = MXFP4.empty(rows, cols, x.device)
         if rows:
@@ -1753,6 +1753,8 @@ class Ops:
                                       f"(shape {tuple(x.shape)}, strides {x.stride()})")
         if K != w.cols:
             raise KernelError(f"{who}: x is {tuple(rows.shape) if not both else (M, K)}, the weight has rows of {w.cols} numbers")
+        if M > MOST or N > MOST:
+            raise KernelError(f"{who}: {M} rows over a weight of {N} rows; the kernels take up to {MOST} of either")
         here = _RAW_DEVICE() if _RAW_DEVICE is not None else torch.cuda.current_device()
         if w.codes.get_device() != here or rows.get_device() != here:
             self._check_here(w.codes, "weight")

@@ -10,6 +10,7 @@ from __future__ import annotations
 import torch
 
 BLOCK = 32
+MOST = 2 ** 30 - 1                 # columns of a matrix, rows of a product: the kernels count them in 32 bits
 
 
 class MXFP4:
@@ -30,6 +31,8 @@ class MXFP4:
         if cols <= 0 or blocks != -(-cols // BLOCK) or code_bytes != blocks * 16 or rows != scale_rows:
             raise ValueError(f"MXFP4: codes {tuple(codes.shape)} and scales {tuple(scales.shape)} do not hold rows of {cols} numbers: "
                              f"{-(-cols // BLOCK)} blocks of 16 bytes and one scale each")
+        if cols > MOST:
+            raise ValueError(f"MXFP4: rows of {cols} numbers; the kernels take up to {MOST}")
         if codes.device != scales.device:
             raise ValueError(f"MXFP4: codes on {codes.device}, scales on {scales.device}")
         (ld_codes, one), (ld_scales, one_too) = codes.stride(), scales.stride()
