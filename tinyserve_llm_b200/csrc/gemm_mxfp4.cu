@@ -11,14 +11,20 @@ static bool few_in_registers(int M, int N, int K, bool both) {
     return (M <= SKINNY_MX_ROWS && numbers <= 5ll << 20) || (!both && M <= 8 && numbers <= 1ll << 24);
 }
 
-// Whether rows in bfloat16 are multiplied as two rows of 8-bit numbers each, with W's codes as they are, and not with W's codes spread to
-// bfloat16: 28,672 by 4,096 gated, 8 rows 18.4 us (spread 40.7), 64 rows 28 (42.6), 96 rows 56 (46); 2,048 by 8,192, 17 to 64 rows 10.3 to
-// 14.0 (13.9 to 15.5); 2,048 by 2,048, 64 rows 9.7 (9.0).  More rows again where wide tiles of them fit the SMs in one round, and spreading,
-// whose tiles are smaller then, would be done over for each: 2,048 by 8,192, 512 rows 25 us (29), 1,024 rows 39 (50); 4,096 by 4,096, 384 rows
-// 22 (28); but 96 rows 23 (17).
+// Whether rows in bfloat16 are multiplied as three rows of 8-bit numbers each, with W's codes as they are, and not with W's codes spread to
+// bfloat16.  Device times on a B200, other weights each time, in pieces (spread): up to 16 rows always, 28,672 by 4,096 gated, 8 and 16 rows
+// 18.8 and 20.1 us (40.7, 38.5), 4,096 by 14,336 14.7 and 17.2 (23.3), 4,096 by 4,096, 16 rows 9.3 (9.5).  Up to 32 rows where there is enough
+// of W or K is long: 28,672 by 4,096 22.7 (39.1), 2,048 by 8,192 12.6 (13.3), but 4,096 by 4,096 10.6 (9.6).  Up to 64 where K is long, N splits in
+// enough tiles that clusters of eight CTAs are not needed, which one CTA an SM leaves no room for, and there is enough of W: 28,672 by 4,096
+// 34.7 (40.2), 4,096 by 14,336 21.3 (24.9), 6,144 by 4,096 14.1 (15.7), but 16,384 by 2,048 16.6 (14.9), 2,048 by 8,192 20.2 (14.4), 4,096 by
+// 4,096 13.4 (10.7).  Beyond, three bytes of x a number are more to bring than spreading costs: 512 rows, 2,048 by 8,192 31.6 (28.3), 4,096 by
+// 4,096 33.1 (26.2).
 static bool in_pieces(int M, int N, int K) {
-    const long long numbers = (long long)N * K, wide_tiles = (long long)((N + 127) / 128) * ((2 * (long long)M + 255) / 256);
-    return K % 128 == 0 && numbers > 5ll << 20 && (M <= 64 || (M > 128 && wide_tiles <= 148));
+    const long long numbers = (long long)N * K;
+    if (K % 128 || numbers <= 5ll << 20) return false;
+    if (M <= 16) return true;
+    if (M <= 32) return K > 4096 || numbers > 1ll << 24;
+    return M <= 64 && K >= 4096 && N > 2304 && numbers > 5ll << 22;
 }
 
 // Bytes of scratch a product may need (16-byte aligned; 0: none).

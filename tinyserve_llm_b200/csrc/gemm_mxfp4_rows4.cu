@@ -6,13 +6,15 @@
 // stage), and put them into a ring of their own in shared memory, of a stage's 16 bytes for lane l bytes 4 j .. 4 j + 3 of row 32 j + l;
 // tcgen05.cp hands them to all four quarters of the lanes.
 //
-// A few rows of bfloat16 numbers take the same way (KIND 8): each row becomes two rows of 8-bit floating point (e4m3, blocks of 32 under a
-// scale of a power of two), the number rounded to four bits and what that left, and tcgen05.mma kind::mxf8f6f4 multiplies them with W's
-// codes as they are; the two products are added up.  Four bits and four make a bfloat16's eight: only of numbers 2^13 times smaller than
-// their block's largest something is lost, less than 2^-21 of that largest.  An MMA of some columns costs next to nothing beside the stream of
-// W, where spreading W's codes to bfloat16, for tensor memory or in registers, takes longer than bringing them (28,672 rows of 4,096, eight
-// rows of x: 41 us).  A block of x with a NaN is NaN.  Infinities have no place in these blocks: one that holds some, and no NaN, is zeros and
-// then NaN, and results whose second piece alone is NaN are worked out again, number by number.
+// A few rows of bfloat16 numbers take the same way (KIND 8): each row becomes three rows of 8-bit floating point (e5m2, blocks of 32 under a
+// scale of a power of two), the number rounded to three bits, what that left, and what that left again, and tcgen05.mma kind::mxf8f6f4
+// multiplies them with W's codes as they are; the three products are added up.  Three bits, their signs and a third piece make a bfloat16's
+// eight, exactly, of numbers down to some 2^31 times smaller than their block's largest.  (Two pieces of e4m3 have the bits, but not the
+// range: they lose some of numbers 2^14 times smaller, and of a norm's output one number in 5,000 is.)  A block with numbers smaller still
+// that are not zero, with infinities or NaNs is zeros in the pieces, under a scale of its own, and multiplied number by number.
+//
+// An MMA of some columns costs next to nothing beside the stream of W, where spreading W's codes to bfloat16, for tensor memory or in
+// registers, takes longer than bringing them (28,672 rows of 4,096, eight rows of x: 41 us).
 #include <cuda_fp16.h>
 
 #include "gemm_mxfp4.cuh"
@@ -45,11 +47,11 @@ __device__ __forceinline__ void umma8(uint32_t leader, uint32_t d, uint64_t a, u
         "@q tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
         ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate), "r"(leader) : "memory");
 }
-// e2m1 x e2m1 -> float32 (KIND 4) with two scales a row and MMA, or e2m1 x e4m3 (KIND 8) with one; scales are power-of-two bytes, `byte`: the
+// e2m1 x e2m1 -> float32 (KIND 4) with two scales a row and MMA, or e2m1 x e5m2 (KIND 8) with one; scales are power-of-two bytes, `byte`: the
 // first of an MMA's in the four bytes of a column.
 template <int KIND>
 __device__ __forceinline__ uint32_t instr_desc(int n, int byte) {
-    return (uint32_t)byte << 4 | (KIND == 4 ? 1u << 7 | 1u << 10 : 5u << 7) | (uint32_t)(n >> 3) << 17 | 1u << 23 | (uint32_t)(BM >> 7) << 27 |
+    return (uint32_t)byte << 4 | (KIND == 4 ? 1u << 7 | 1u << 10 : 5u << 7 | 1u << 10) | (uint32_t)(n >> 3) << 17 | 1u << 23 | (uint32_t)(BM >> 7) << 27 |
            (uint32_t)byte << 29;
 }
 
@@ -58,7 +60,25 @@ __host__ __device__ constexpr int x_sets() { return (BN + 127) / 128; }         
 template <int KIND, int BN>
 __host__ __device__ constexpr int scale_columns() { return (KIND == 4 ? 8 : 4) * (1 + x_sets<BN>()); }        // of tensor memory, a stage
 
-constexpr int PIECES8 = 2;                             // rows of e4m3 numbers a row of bfloat16 ones becomes
+constexpr int PIECES8 = 3;                             // rows of e5m2 numbers a row of bfloat16 ones becomes
+constexpr uint32_t BY_HAND = 254;                      // scale of a block that is not in the pieces: no other block has it
+// Rows of x in a tile whose MMAs have BN columns: its first pieces, then the second, then the third.  (32 columns: 24 and eight nobody reads.)
+template <int KIND, int BN>
+__host__ __device__ constexpr int tile_rows() { return KIND == 4 ? BN : BN == 32 ? 8 : BN / PIECES8; }
+
+__device__ __forceinline__ void tma_load_3d(void* smem, const CUtensorMap* map, uint64_t* bar, int x, int y, int z) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+        ::"r"(smem_u32(smem)), "l"(map), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z) : "memory");
+}
+__device__ __forceinline__ void tmem_ld8(uint32_t addr, uint32_t (&r)[8]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void tmem_wait8(uint32_t (&r)[8]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7])::"memory");
+}
 
 // One product of a row of W with a bfloat16 row of x, number by number.
 __device__ __noinline__ float plain_dot(const uint8_t* codes, const uint8_t* scales, const __nv_bfloat16* x, int K) {
@@ -73,37 +93,75 @@ __device__ __forceinline__ float plain_dot(const MxParams& p, int row, int t) {
     return plain_dot(p.w_codes + row * p.w_ld_codes, p.w_scales + row * p.w_ld_scales, p.x16 + t * p.x16_ld, p.K);
 }
 
-// A result from its two pieces' products; infinite (whatever its sign) stands for one that has to be worked out again.
-__device__ __forceinline__ float added(float first, float second) {
-    return second != second && first == first ? __int_as_float(0x7f800000) : first + second;
+// What the blocks that are not in the pieces, from `block0` to `block1` (multiples of four), add to the product of a lane's row of W with a row of
+// x, whose first pieces' scales are `x_scales`.
+__device__ __noinline__ float by_hand(const uint8_t* codes, const uint8_t* scales, const __nv_bfloat16* x, const uint8_t* x_scales, int block0,
+                                      int block1, int lane) {
+    float sum = 0.f;
+    for (int b0 = block0; b0 < block1; b0 += 128) {                   // a lane looks at four blocks' scales
+        const int four = b0 + lane * 4;
+        const uint32_t word = four < block1 ? __ldg(reinterpret_cast<const uint32_t*>(x_scales + four)) : 0;
+        const uint32_t mine = __vcmpeq4(word, BY_HAND * 0x01010101u);
+        for (uint32_t who = __ballot_sync(0xffffffffu, mine != 0); who; who &= who - 1) {
+            const int l = __ffs(who) - 1;
+            for (uint32_t left = __shfl_sync(0xffffffffu, mine, l) & 0x01010101u; left; left &= left - 1) {
+                const int block = b0 + l * 4 + (__ffs(left) - 1) / 8;
+                const uint4 code = __ldg(reinterpret_cast<const uint4*>(codes + block * 16ll));
+                const float scale = mx_scale(__ldg(scales + block));
+                const float number = to_float(x[block * 32ll + lane]);
+                const uint32_t words[4] = {code.x, code.y, code.z, code.w};
+#pragma unroll
+                for (int e = 0; e < 32; ++e)
+                    sum = fmaf(mx_code_value(words[e >> 3] >> (4 * (e & 7)) & 15) * scale, __shfl_sync(0xffffffffu, number, e), sum);
+            }
+        }
+    }
+    return sum;
 }
 
-// The columns of a tile whose x came in two pieces a row: an epilogue warp's share, 16 columns, eight rows of x, at a time.
-template <bool GATED, int SHARE>
-__device__ __forceinline__ void finish_pieces(const MxParams& p, uint32_t tmem, int first, int t0, int f0, int outs, int quarter, int lane,
-                                              float* sums) {
-    const uint32_t addr = tmem + first + ((uint32_t)(quarter * 32) << 16);
+// The columns of a tile whose x came in pieces, eight rows of x at a time: an epilogue warp takes every other eight (`half`).  `marked`: a bit
+// for each of the tile's rows that has blocks, of its CTA's, to be multiplied by hand.
+template <bool GATED, int ROWS>
+__device__ __forceinline__ void finish_pieces(const MxParams& p, uint32_t tmem, int half, int t0, int f0, int outs, int quarter, int lane, float* sums,
+                                              const uint32_t* marked, int block0, int block1) {
+    const uint32_t addr = tmem + ((uint32_t)(quarter * 32) << 16);
     const int f = GATED ? f0 + quarter * 16 + (lane & 15) : f0 + quarter * 32 + lane;
+    const int row = min(row_of<GATED>(p, f0, quarter * 32 + lane), p.N - 1);
 #pragma unroll 1
-    for (int c0 = 0; c0 < SHARE; c0 += 16) {
-        uint32_t acc[16];
+    for (int r = half * 8; r < ROWS; r += 16) {
+        const int t = t0 + r;
+        if (t >= p.M) break;
+        uint32_t acc[PIECES8][8];
         __syncwarp();
-        tmem_ld16(addr + c0, acc);
-        tmem_wait16(acc);
-        const int column = (first + c0) / PIECES8, t = t0 + column;
-        float v[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = added(__uint_as_float(acc[2 * j]), __uint_as_float(acc[2 * j + 1]));
+        for (int i = 0; i < PIECES8; ++i) tmem_ld8(addr + i * ROWS + r, acc[i]);
+#pragma unroll
+        for (int i = 0; i < PIECES8; ++i) tmem_wait8(acc[i]);
+        float v[8];
+        uint32_t past = 0;                                            // the first pieces, rounded up, may leave float32's range alone
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            v[j] = __uint_as_float(acc[0][j]) + (__uint_as_float(acc[1][j]) + __uint_as_float(acc[2][j]));
+            past |= (isinf(v[j]) ? 1u : 0u) << j;
+        }
+        const uint32_t some = marked[r >> 5] >> (r & 31) & 0xff;
+        if (some) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if ((some >> j & 1) && t + j < p.M)
+                    v[j] += by_hand(p.w_codes + row * p.w_ld_codes, p.w_scales + row * p.w_ld_scales, p.x16 + (t + j) * p.x16_ld,
+                                    p.x_scales + (t + j) * p.x_ld_scales, block0, block1, lane);
+        }
         if (p.splits > 1) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) sums[(column + j) * BM + quarter * 32 + lane] = v[j];
+            for (int j = 0; j < 8; ++j) sums[(r + j) * BM + quarter * 32 + lane] = v[j];
             continue;
         }
-        if (t >= p.M) continue;
-        const int row = row_of<GATED>(p, f0, quarter * 32 + lane);
+        if (past) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-            if (isinf(v[j]) && t + j < p.M && row < p.N) v[j] = plain_dot(p, row, t + j);
+            for (int j = 0; j < 8; ++j)
+                if ((past >> j & 1) && t + j < p.M) v[j] = plain_dot(p, row, t + j);
+        }
         __syncwarp();
         if (GATED) {                                                  // the lower half of the lanes finishes even rows of x, the upper one odd ones
 #pragma unroll
@@ -138,26 +196,27 @@ __host__ __device__ constexpr int ring_bytes() {
 template <int KIND, bool GATED, int BN, int STAGES, bool SPLIT>
 __global__ void __launch_bounds__(THREADS, ring_bytes<KIND, BN, STAGES>() <= 113 * 1024 ? 2 : 1)
 rows4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, MxParams p) {
-    constexpr int PIECES = KIND == 4 ? 1 : PIECES8, CHUNK = KIND == 4 ? 256 : 128;      // columns of K in the 128 bytes of a row and stage
+    constexpr int ROWS = tile_rows<KIND, BN>(), CHUNK = KIND == 4 ? 256 : 128;      // columns of K in the 128 bytes of a row and stage
     constexpr int SETS = KIND == 4 ? 2 : 1;          // of four scales a row and stage
     constexpr int GROUP_BITS = group_bits<KIND>(), PER_GROUP = 1 << GROUP_BITS, GROUPS_HELD = groups_held<KIND>();
     constexpr int B_BYTES = BN * ROW, SCALE_COLS = scale_columns<KIND, BN>(), SCALE_BYTES = SCALE_COLS * 128, X_SETS = x_sets<BN>();
     constexpr int ACCUMULATORS = SPLIT ? 1 : 2, OUTS = GATED ? BM / 2 : BM, SHARE = BN / (EPI_WARPS / 4);
     constexpr int TMEM_USED = ACCUMULATORS * BN + STAGES * SCALE_COLS, TMEM_COLS = power_of_two(TMEM_USED);
     static_assert(TMEM_USED <= 512, "tensor memory has 512 columns");
-    static_assert(PIECES == 1 || SPLIT, "pieces are added up by tiles");
-    static_assert(!SPLIT || BM * BN / PIECES * 4 <= STAGES * (A_BYTES + B_BYTES), "a split tile's sums go where the ring was");
+    static_assert(KIND == 4 || SPLIT, "pieces are added up by tiles");
+    static_assert(KIND == 4 || (ROWS % 8 == 0 && ROWS <= 64 && ROWS * PIECES8 <= BN), "eights of rows, a bit each in two words");
+    static_assert(!SPLIT || BM * ROWS * 4 <= STAGES * (A_BYTES + B_BYTES), "a split tile's sums go where the ring was");
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     __shared__ __align__(8) uint64_t full_bar[STAGES], empty_bar[STAGES], tmem_full_bar[2], tmem_empty_bar[2];
     __shared__ __align__(8) uint64_t scales_full[GROUPS_HELD], scales_empty[GROUPS_HELD];
-    __shared__ uint32_t tmem_base_slot;
+    __shared__ uint32_t tmem_base_slot, marked[2];
     __shared__ int failed;
 
     unsigned char* stages = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     unsigned char* scale_ring = stages + STAGES * (A_BYTES + B_BYTES);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int outs = GATED ? p.inter : p.N;
-    const int x_tiles = (p.M * PIECES + BN - 1) / BN, num_tiles = x_tiles * ((outs + OUTS - 1) / OUTS);
+    const int x_tiles = (p.M + ROWS - 1) / ROWS, num_tiles = x_tiles * ((outs + OUTS - 1) / OUTS);
     const int all_chunks = (p.blocks * MX_BLOCK + CHUNK - 1) / CHUNK;
     const int rank = SPLIT && p.splits > 1 ? (int)pair_rank() : 0;
     const int first_tile = SPLIT ? (int)blockIdx.x / p.splits : (int)blockIdx.x, tile_step = SPLIT ? num_tiles : (int)gridDim.x;
@@ -177,6 +236,7 @@ rows4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
             mbar_init(&tmem_full_bar[b], 1);
             mbar_init(&tmem_empty_bar[b], EPI_WARPS);
         }
+        marked[0] = marked[1] = 0;
         failed = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -197,14 +257,15 @@ rows4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
         if (lane == 0) {
             Ring<STAGES> r;
             for (int tile = first_tile; tile < num_tiles && !failed; tile += tile_step) {
-                const int t0 = (tile % x_tiles) * (BN / PIECES), f0 = (tile / x_tiles) * OUTS;
+                const int t0 = (tile % x_tiles) * ROWS, f0 = (tile / x_tiles) * OUTS;
                 for (int chunk = chunk0; chunk < chunk1; ++chunk, r.next()) {
                     const int s = r.at;
                     if (!wait_for(&empty_bar[s], r.parity ^ 1, p.error, 41)) { failed = 1; break; }
                     unsigned char* tile_at = stages + s * (A_BYTES + B_BYTES);
-                    mbar_expect_tx(&full_bar[s], (KIND == 4 ? A_BYTES : A_BYTES / 2) + B_BYTES);      // spaced codes count without the space
+                    mbar_expect_tx(&full_bar[s], KIND == 4 ? A_BYTES + B_BYTES : A_BYTES / 2 + ROWS * PIECES8 * ROW);       // spaced codes count without the space
                     load_codes<GATED>(tile_at, &map_w, &full_bar[s], p, chunk * ROW, f0);
-                    tma_load_2d(tile_at + A_BYTES, &map_x, &full_bar[s], chunk * ROW, t0 * PIECES);
+                    if (KIND == 4) tma_load_2d(tile_at + A_BYTES, &map_x, &full_bar[s], chunk * ROW, t0);
+                    else tma_load_3d(tile_at + A_BYTES, &map_x, &full_bar[s], chunk * ROW, t0, 0);
                 }
             }
         }
@@ -259,32 +320,41 @@ rows4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
         int iter = 0;
         for (int tile = first_tile; tile < num_tiles; tile += tile_step, ++iter) {
             const int buf = SPLIT ? 0 : iter & 1;
-            const int t0 = (tile % x_tiles) * (BN / PIECES), f0 = (tile / x_tiles) * OUTS;
+            const int t0 = (tile % x_tiles) * ROWS, f0 = (tile / x_tiles) * OUTS;
             const bool ok = wait_for(&tmem_full_bar[buf], (iter >> 1) & 1, p.error, 43) && !failed;
             if (!__all_sync(0xffffffffu, ok)) { failed = 1; break; }
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            if (PIECES > 1)
-                finish_pieces<GATED, SHARE>(p, tmem_base, first, t0, f0, outs, quarter, lane, reinterpret_cast<float*>(stages));
-            else
+            if constexpr (KIND == 8) {
+                // what the warps of the scales have marked is there when they have handed on their last ones
+                const int groups = ((chunk1 - 1) >> GROUP_BITS) - (chunk0 >> GROUP_BITS);
+                if (!__all_sync(0xffffffffu, wait_for(&scales_full[groups % GROUPS_HELD], (groups / GROUPS_HELD) & 1, p.error, 43))) { failed = 1; break; }
+                finish_pieces<GATED, ROWS>(p, tmem_base, (warp - 2) >> 2, t0, f0, outs, quarter, lane, reinterpret_cast<float*>(stages),
+                                                           marked, chunk0 * 4, chunk1 * 4);
+            } else {
                 finish_tile<GATED, SHARE, SPLIT>(p, tmem_base + buf * BN, first, t0, f0, outs, paired, quarter, lane, reinterpret_cast<float*>(stages),
                                                  &tmem_empty_bar[buf]);
+            }
         }
     } else {
         // ---------------------------------------------------------------- scales
         // Groups of 32 rows, a row a lane: 0 to 3 of W, from 4 on of x; a warp has every fourth.  What a group leaves out of its 512 bytes
         // (fewer than 128 rows of x) belongs to columns that no MMA reads.
-        constexpr int GROUPS = 4 + BN / 32, MINE = (GROUPS + GATHER - 1) / GATHER;
+        constexpr int GROUPS = 4 + (BN + 31) / 32, MINE = (GROUPS + GATHER - 1) / GATHER;
         const int w = warp - 2 - EPI_WARPS;
+        auto x_row = [&](int t0, int n) -> long long {                // of the matrix of x's scales, for row n of a tile
+            if (KIND == 4) return min(t0 + n, p.M - 1);
+            return (long long)min(n / ROWS, PIECES8 - 1) * p.M + min(t0 + n % ROWS, p.M - 1);
+        };
         bool ok = true;
         Ring<GROUPS_HELD> r;
         for (int tile = first_tile; tile < num_tiles && ok; tile += tile_step) {
-            const int t0 = (tile % x_tiles) * (BN / PIECES), f0 = (tile / x_tiles) * OUTS;
+            const int t0 = (tile % x_tiles) * ROWS, f0 = (tile / x_tiles) * OUTS;
             const uint8_t* row[MINE];
 #pragma unroll
             for (int i = 0; i < MINE; ++i) {
                 const int g = w + i * GATHER;
                 row[i] = g < 4 ? p.w_scales + (long long)min(row_of<GATED>(p, f0, g * 32 + lane), p.N - 1) * p.w_ld_scales
-                               : p.x_scales + (long long)min(t0 * PIECES + (g - 4) * 32 + lane, p.M * PIECES - 1) * p.x_ld_scales;
+                               : p.x_scales + x_row(t0, (g - 4) * 32 + lane) * p.x_ld_scales;
             }
             auto load = [&](int group, uint4 (&v)[MINE]) {            // 16 scales of each row; behind the last block 1
                 const int b = group * 16;
@@ -313,6 +383,11 @@ rows4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
                 for (int i = 0; i < MINE; ++i) {
                     const int g = w + i * GATHER;
                     if (g >= GROUPS) continue;
+                    if (KIND == 8 && g >= 4 && (g - 4) * 32 < ROWS) {             // the tile's rows, a lane each: which are to be multiplied by hand
+                        const uint32_t hand = BY_HAND * 0x01010101u;
+                        if (__vcmpeq4(now[i].x, hand) | __vcmpeq4(now[i].y, hand) | __vcmpeq4(now[i].z, hand) | __vcmpeq4(now[i].w, hand))
+                            if ((g - 4) * 32 + lane < ROWS) atomicOr(&marked[(g - 4) & 1], 1u << lane);
+                    }
                     // word j of the row: stage j / SETS of the group, set j % SETS
                     const int of_x = g < 4 ? 0 : SETS * 512 + ((g - 4) >> 2) * 512;
                     unsigned char* to = scale_ring + r.at * PER_GROUP * SCALE_BYTES + of_x + lane * 16 + (g & 3) * 4;
@@ -333,9 +408,9 @@ rows4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
     __syncwarp();
     if (SPLIT && p.splits > 1) {
         pair_sync();                                 // every CTA's sums are in its shared memory
-        const int t0 = (first_tile % x_tiles) * (BN / PIECES), f0 = (first_tile / x_tiles) * OUTS;
-        const auto again = [&](int l, int t, float v) { return PIECES > 1 && isinf(v) ? plain_dot(p, min(row_of<GATED>(p, f0, l), p.N - 1), t) : v; };
-        join_splits<GATED>(p, smem_u32(stages), rank, min(BN / PIECES, p.M - t0), t0, f0, outs, threadIdx.x, THREADS, again);
+        const int t0 = (first_tile % x_tiles) * ROWS, f0 = (first_tile / x_tiles) * OUTS;
+        const auto again = [&](int l, int t, float v) { return KIND == 8 && isinf(v) ? plain_dot(p, min(row_of<GATED>(p, f0, l), p.N - 1), t) : v; };
+        join_splits<GATED>(p, smem_u32(stages), rank, min(ROWS, p.M - t0), t0, f0, outs, threadIdx.x, THREADS, again);
         __syncwarp();
         pair_sync();                                 // nobody reads another CTA's sums any more
     }
@@ -351,9 +426,9 @@ rows4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
     }
 }
 
-// bfloat16 rows as two rows of e4m3 numbers each, m * 2 and m * 2 + 1.  Four lanes a block, eight numbers a lane.
+// bfloat16 rows as three rows of e5m2 numbers each: all first pieces, all second ones, all third ones.  Four lanes a block, eight numbers a lane.
 __global__ void __launch_bounds__(256) pieces_kernel(const __nv_bfloat16* __restrict__ x, long long ldx, uint2* __restrict__ numbers,
-                                                     uint8_t* __restrict__ scales, int M, int K, int blocks, int ld_scales) {
+                                                     uint8_t* __restrict__ scales, int M, int blocks, int ld_scales) {
     chain_wait();
     chain_release();
     const int lanes = blocks * 4;
@@ -362,15 +437,13 @@ __global__ void __launch_bounds__(256) pieces_kernel(const __nv_bfloat16* __rest
     const bool mine = at < total;
     const int m = mine ? (int)(at / lanes) : 0, part = mine ? (int)(at - (long long)m * lanes) : 0;
     float v[8];
-    if (mine && part * 8 < K) {                                       // K is a multiple of 8
-        const uint4 q = *reinterpret_cast<const uint4*>(x + (long long)m * ldx + part * 8);
-        const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+    const uint4 q = mine ? *reinterpret_cast<const uint4*>(x + (long long)m * ldx + part * 8) : make_uint4(0, 0, 0, 0);
+    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[2 * i] = __uint_as_float(w[i] << 16), v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = 0.f;
-    }
+    for (int i = 0; i < 4; ++i) v[2 * i] = __uint_as_float(w[i] << 16), v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    uint2 packed[PIECES8];
+    int scale_byte[PIECES8];
+    bool hand = false;                                                // not finite, or something is left of it
 #pragma unroll
     for (int i = 0; i < PIECES8; ++i) {
         uint32_t top = 0;
@@ -378,37 +451,35 @@ __global__ void __launch_bounds__(256) pieces_kernel(const __nv_bfloat16* __rest
         for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(v[e]) & 0x7fffffffu);       // what is not finite is largest
         top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        // the largest becomes a number from 128 to 256, of 448 that there is room for
-        const int exponent = (int)(top >> 23);
-        int s = exponent == 255 ? 255 : max(exponent - 7, 0);
-        uint2 packed = make_uint2(0, 0);
-        if (exponent != 255) {
-            const float inverse = __uint_as_float((uint32_t)(254 - s) << 23), scale = mx_scale(s);
-            uint32_t two[4];
+        if (i == 0) hand = top >= 0x7f800000u;
+        // the largest becomes a number from 2^14 to 2^15, of 1.75 2^15 that there is room for
+        const int s = max((int)(top >> 23) - 14, 0);
+        const float inverse = __uint_as_float((uint32_t)(254 - s) << 23), scale = mx_scale(s);
+        uint32_t two[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                uint16_t codes;
-                uint32_t halves;
-                asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(codes) : "f"(v[2 * e + 1] * inverse), "f"(v[2 * e] * inverse));
-                asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(halves) : "h"(codes));
-                const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&halves));
-                v[2 * e] -= back.x * scale;                           // exact: a bfloat16 less its leading bits
-                v[2 * e + 1] -= back.y * scale;
-                two[e] = codes;
-            }
-            packed = make_uint2(two[0] | two[1] << 16, two[2] | two[3] << 16);
-        } else {
-            if (i == 0 && top == 0x7f800000u) {
-                s = 0;                                                // infinities and no NaN: the second piece is NaN
-            } else {
+        for (int e = 0; e < 4; ++e) {
+            uint16_t codes;
+            uint32_t halves;
+            asm("cvt.rn.satfinite.e5m2x2.f32 %0, %1, %2;" : "=h"(codes) : "f"(v[2 * e + 1] * inverse), "f"(v[2 * e] * inverse));
+            asm("cvt.rn.f16x2.e5m2x2 %0, %1;" : "=r"(halves) : "h"(codes));
+            const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&halves));
+            v[2 * e] -= back.x * scale;                               // exact: a bfloat16 less its leading bits
+            v[2 * e + 1] -= back.y * scale;
+            two[e] = codes;
+        }
+        packed[i] = make_uint2(two[0] | two[1] << 16, two[2] | two[3] << 16);
+        scale_byte[i] = s;
+    }
 #pragma unroll
-                for (int e = 0; e < 8; ++e) v[e] = 0.f;
-            }
-        }
-        if (mine) {
-            numbers[((long long)m * PIECES8 + i) * lanes + part] = packed;
-            if ((part & 3) == 0) scales[((long long)m * PIECES8 + i) * ld_scales + (part >> 2)] = (uint8_t)s;
-        }
+    for (int e = 0; e < 8; ++e) hand |= v[e] != 0.f;
+    const uint32_t block_lanes = 0xfu << (threadIdx.x & 28);
+    hand = (__ballot_sync(0xffffffffu, hand) & block_lanes) != 0;     // any of the block's
+    if (!mine) return;
+#pragma unroll
+    for (int i = 0; i < PIECES8; ++i) {
+        const long long row = (long long)i * M + m;
+        numbers[row * lanes + part] = hand ? make_uint2(0, 0) : packed[i];
+        if ((part & 3) == 0) scales[row * ld_scales + (part >> 2)] = (uint8_t)(hand ? BY_HAND : scale_byte[i]);
     }
 }
 
@@ -416,8 +487,16 @@ template <int KIND, bool GATED, int BN, int STAGES, bool SPLIT>
 int run(const void* x, long long ldx, MxParams& p, long long tiles, int sms, int device, cudaStream_t stream) {
     CUtensorMap map_w, map_x;
     if (make_codes_map<GATED>(&map_w, p, KIND == 8)) return 1;
-    const long long rows = (long long)p.M * (KIND == 4 ? 1 : PIECES8), bytes = (long long)p.blocks * (KIND == 4 ? 16 : 32);
-    if (make_tile_map(&map_x, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, x, rows, bytes, ldx, BN, "gemm_mxfp4")) return 1;
+    if (KIND == 4) {
+        if (make_tile_map(&map_x, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, x, p.M, p.blocks * 16ll, ldx, BN, "gemm_mxfp4")) return 1;
+    } else {                                         // bytes, rows, pieces
+        const cuuint64_t dims[3] = {(cuuint64_t)ldx, (cuuint64_t)p.M, PIECES8}, strides[2] = {(cuuint64_t)ldx, (cuuint64_t)ldx * p.M};
+        const cuuint32_t box[3] = {ROW, (cuuint32_t)tile_rows<KIND, BN>(), PIECES8}, elem[3] = {1, 1, 1};
+        const CUresult r = encode_tiled()(&map_x, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(x), dims, strides, box, elem,
+                                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+        if (r != CUDA_SUCCESS) return ts_fail("gemm_mxfp4: cuTensorMapEncodeTiled failed with %d", (int)r);
+    }
     static unsigned long long allowed = 0;
     return launch_mxfp4(rows4_kernel<KIND, GATED, BN, STAGES, SPLIT>, allowed, THREADS, (size_t)ring_bytes<KIND, BN, STAGES>() + 1024, SPLIT, tiles, sms,
                         device, map_w, map_x, p, stream);
@@ -441,14 +520,16 @@ template <bool GATED>
 int dispatch_pieces(const void* numbers, MxParams& p, cudaStream_t stream) {
     int sms = 148, device = 0;
     if (cudaGetDevice(&device) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
-    const int rows = p.M * PIECES8, bn = rows <= 32 ? 32 : rows <= 64 ? 64 : rows <= 128 ? 128 : 256;
     const long long ldx = (long long)p.blocks * 32;
-    const long long outs = GATED ? p.inter : p.N, per = GATED ? BM / 2 : BM, tiles = (outs + per - 1) / per * ((rows + bn - 1) / bn);
+    const long long outs = GATED ? p.inter : p.N, per = GATED ? BM / 2 : BM, tiles = (outs + per - 1) / per;
     p.splits = splits_of(p, tiles, sms);
-    if (bn == 32) return run<8, GATED, 32, 5, true>(numbers, ldx, p, tiles, sms, device, stream);
-    if (bn == 64) return run<8, GATED, 64, 4, true>(numbers, ldx, p, tiles, sms, device, stream);
-    if (bn == 128) return run<8, GATED, 128, 3, true>(numbers, ldx, p, tiles, sms, device, stream);
-    return run<8, GATED, 256, 4, true>(numbers, ldx, p, tiles, sms, device, stream);
+    if (p.M <= 8) return run<8, GATED, 32, 5, true>(numbers, ldx, p, tiles, sms, device, stream);
+    if (p.M <= 16) return run<8, GATED, 48, 4, true>(numbers, ldx, p, tiles, sms, device, stream);
+    if (p.M <= 32) return run<8, GATED, 96, 3, true>(numbers, ldx, p, tiles, sms, device, stream);
+    // more tiles than SMs: two CTAs an SM, with what is left of a ring each (28,672 by 4,096 gated, 64 rows 34.7 us, 40.8 one behind the other);
+    // else one (6,144 by 4,096 14.1 and 18.7)
+    if (tiles > sms) return run<8, GATED, 192, 2, true>(numbers, ldx, p, tiles, sms, device, stream);
+    return run<8, GATED, 192, 4, true>(numbers, ldx, p, tiles, sms, device, stream);
 }
 
 }  // namespace
@@ -461,7 +542,7 @@ bool mxfp4_takes_pieces(const void* w_codes, long long w_ld_codes, int K) {
     return K % 128 == 0 && w_ld_codes % 32 == 0 && (uintptr_t)w_codes % 32 == 0;      // what TMA asks of 4-bit numbers that it spaces out
 }
 
-long long mxfp4_pieces_bytes(int M, int blocks) { return (long long)M * PIECES8 * (blocks * 32 + (blocks + 15) / 16 * 16); }
+long long mxfp4_pieces_bytes(int M, int blocks) { return (long long)M * PIECES8 * (blocks * 32ll + (blocks + 15) / 16 * 16); }
 
 int mxfp4_pieces(const void* x, long long ldx, void* scratch, MxParams& p, int gated, cudaStream_t stream) {
     uint8_t* numbers = (uint8_t*)scratch;
@@ -472,6 +553,6 @@ int mxfp4_pieces(const void* x, long long ldx, void* scratch, MxParams& p, int g
     p.x16_ld = ldx;
     const dim3 grid((unsigned)(((long long)p.M * p.blocks * 4 + 255) / 256));
     TS_CHAINED_CHECK("gemm_mxfp4", launch_chained(pieces_kernel, grid, dim3(256), 0, stream, (const __nv_bfloat16*)x, ldx, (uint2*)numbers, scales,
-                                                  p.M, p.K, p.blocks, (int)p.x_ld_scales));
+                                                  p.M, p.blocks, (int)p.x_ld_scales));
     return gated ? dispatch_pieces<true>(numbers, p, stream) : dispatch_pieces<false>(numbers, p, stream);
 }
