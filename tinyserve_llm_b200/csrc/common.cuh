@@ -52,16 +52,28 @@ __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { re
 template <typename T>
 __device__ __forceinline__ float round_to(float v) { return to_float<T>(from_float<T>(v)); }
 
+// The smaller and the larger of two numbers, NaN if either is one, which fminf and fmaxf would drop.
+__device__ __forceinline__ float ts_min(float a, float b) {
+    float d;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    return d;
+}
+__device__ __forceinline__ float ts_max(float a, float b) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    return d;
+}
+
 // Gated activations of feed-forward layers, act(gate, up):  0: silu(g) u;  1: relu(g) u;
 // 2: g' sigmoid(alpha g') (u' + 1) with g' = min(g, limit), u' = clamp(u, -limit, limit);
 // 3: gelu(g) u in the tanh form, gelu(g) = g/2 (1 + tanh(sqrt(2/pi) (g + 0.044715 g^3))).
 enum { TS_ACT_SILU = 0, TS_ACT_RELU = 1, TS_ACT_CLAMPED_SWISH = 2, TS_ACT_GELU_TANH = 3, TS_ACT_LAST = TS_ACT_GELU_TANH };
 
 __device__ __forceinline__ float ts_gated_activation(int kind, float g, float u, float limit, float alpha) {
-    if (kind == TS_ACT_RELU) return fmaxf(g, 0.f) * u;
+    if (kind == TS_ACT_RELU) return ts_max(g, 0.f) * u;
     if (kind == TS_ACT_CLAMPED_SWISH) {
-        g = fminf(g, limit);
-        u = fminf(fmaxf(u, -limit), limit);
+        g = ts_min(g, limit);
+        u = ts_min(ts_max(u, -limit), limit);
         return g / (1.f + expf(-alpha * g)) * (u + 1.f);
     }
     if (kind == TS_ACT_GELU_TANH)
