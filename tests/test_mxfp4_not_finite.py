@@ -95,3 +95,38 @@ def test_nans_through_the_activation_alone(ops, act, dtype):
         want = np.zeros((m, 256), dtype=bool)
         want[1], want[:, 3] = True, True
         np.testing.assert_array_equal(np.isnan(y), want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["relu2", "xielu", "tanh"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_nans_through_activations_of_one_argument(ops, dtype, kind):
+    """The elementwise kernel, products with the activation in their epilogue and not, and a projection held in four bits."""
+    from tinyserve_llm_b200.parts.base import Runtime
+    from tinyserve_llm_b200.parts.linear import QuantizedLinear
+    z = numbers((3, 40), dtype, 5)
+    z[0, 2], z[1, 0] = float("nan"), float("nan")
+    np.testing.assert_array_equal(np.isnan(f64(ops.unary_activation(z.to(DEV), kind, 0.8, 0.8))), np.isnan(f64(z)))
+    for m in (4, 40, 300):
+        x, w = numbers((m, 128), dtype, 6).to(DEV), numbers((256, 128), dtype, 7).to(DEV)
+        x[1, 5] = float("nan")
+        w[3, 5] = float("nan")
+        want = np.zeros((m, 256), dtype=bool)
+        want[1], want[:, 3] = True, True
+        np.testing.assert_array_equal(np.isnan(f64(ops.linear_unary(x, w, kind, 0.8, 0.8))), want)
+        if dtype == torch.bfloat16:
+            held_in_four = QuantizedLinear(w, Runtime(torch.bfloat16, torch.device(DEV), ops, weight_format="mxfp4"))
+            np.testing.assert_array_equal(np.isnan(f64(held_in_four.unary(x, kind, 0.8, 0.8))), want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("pairs", [3, 40, 2000])
+def test_nans_through_squares_of_experts(ops, pairs, dtype):
+    x, w = numbers((pairs, 64), dtype, 8).to(DEV), numbers((2, 48, 64), dtype, 9).to(DEV)
+    x[1, 5] = float("nan")
+    offsets = torch.tensor([0, pairs // 2 + 1, pairs], dtype=torch.int32, device=DEV)
+    got = f64(ops.moe_linear(x, w, offsets, None, 1, pairs, "relu2"))
+    want = np.zeros((pairs, 48), dtype=bool)
+    want[1] = True
+    np.testing.assert_array_equal(np.isnan(got), want)

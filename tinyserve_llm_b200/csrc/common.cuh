@@ -86,11 +86,15 @@ __device__ __forceinline__ float ts_gated_activation(int kind, float g, float u,
 // 2: tanh(z).
 enum { TS_UNARY_RELU2 = 0, TS_UNARY_XIELU = 1, TS_UNARY_TANH = 2, TS_UNARY_LAST = TS_UNARY_TANH };
 
+__device__ __forceinline__ float ts_square_of_positive(float z) {
+    const float r = ts_max(z, 0.f);
+    return r * r;
+}
+
 __device__ __forceinline__ float ts_unary_activation(int kind, float z, float a, float b) {
     if (kind == TS_UNARY_XIELU) return z > 0.f ? fmaf(a * z, z, 0.5f * z) : fmaf(b, expm1f(z) - z, 0.5f * z);
     if (kind == TS_UNARY_TANH) return tanhf(z);
-    const float r = fmaxf(z, 0.f);
-    return r * r;
+    return ts_square_of_positive(z);
 }
 
 __device__ __forceinline__ float warp_sum(float v) {

@@ -438,7 +438,7 @@ moe_linear_kernel(const T* __restrict__ x, long long x_stride, const int* __rest
             const int gc = col0 + tc + j;
             if (gc >= out_cols) continue;
             float v = GATED ? ts_gated_activation(kind, acc[i][j], accu[i][j], limit, alpha) : acc[i][j] * rows_scale[tr + i];
-            if (!GATED && unary == 1) v = fmaxf(v, 0.f) * fmaxf(v, 0.f);
+            if (!GATED && unary == 1) v = ts_square_of_positive(v);
             dst[gc] = from_float<T>(v);
         }
     }
@@ -560,7 +560,7 @@ moe_linear_rows_kernel(const T* __restrict__ x, long long x_stride, const int* _
                 const float usum = GATED ? warp_sum(accu[GATED ? g : 0][r]) : 0.f;
                 if (lane == 0) {
                     float v = GATED ? ts_gated_activation(kind, gsum, usum, limit, alpha) : gsum * rows_scale[r];
-                    if (!GATED && unary == 1) v = fmaxf(v, 0.f) * fmaxf(v, 0.f);
+                    if (!GATED && unary == 1) v = ts_square_of_positive(v);
                     y[(long long)(row0 + r) * out_cols + col] = from_float<T>(v);
                 }
             }
@@ -642,7 +642,7 @@ moe_linear_rows_mma_kernel(const __nv_bfloat16* __restrict__ x, long long x_stri
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             float s = acc[i + 2 * h] * scale;
-            if (unary == 1) s = fmaxf(s, 0.f) * fmaxf(s, 0.f);
+            if (unary == 1) s = ts_square_of_positive(s);
             if (col0 + g + 8 * h < out_cols) dst[8 * h] = __float2bfloat16_rn(s);
         }
     }
@@ -846,13 +846,13 @@ __global__ void row_scaled_activation_kernel(const T* __restrict__ x, const int*
 #pragma unroll
             for (int i = 0; i < VN; ++i) {
                 float f = to_float<T>(v[i]) * c;
-                if (unary == 1) f = fmaxf(f, 0.f) * fmaxf(f, 0.f);
+                if (unary == 1) f = ts_square_of_positive(f);
                 v[i] = from_float<T>(f);
             }
             *reinterpret_cast<uint4*>(out + idx) = raw;
         } else {
             float f = to_float<T>(x[idx]) * c;
-            if (unary == 1) f = fmaxf(f, 0.f) * fmaxf(f, 0.f);
+            if (unary == 1) f = ts_square_of_positive(f);
             out[idx] = from_float<T>(f);
         }
     }
