@@ -27,9 +27,10 @@ static bool in_pieces(int M, int N, int K) {
     return M <= 64 && K >= 4096 && N > 2304 && numbers > 5ll << 22;
 }
 
-// Bytes of scratch a product may need (16-byte aligned; 0: none).
-TS_API long long ts_gemm_mxfp4_scratch_bytes(int M, int N, int K, int both) {
-    if (both || M <= 0 || N <= 0 || K <= 0 || few_in_registers(M, N, K, false) || !in_pieces(M, N, K)) return 0;
+// Bytes of scratch a product needs (16-byte aligned), 0 if its rows do not go in pieces.  `spaced`: W's rows of codes start 32-byte aligned, as
+// TMA asks of 4-bit numbers that it spaces out.
+TS_API long long ts_gemm_mxfp4_scratch_bytes(int M, int N, int K, int both, int spaced) {
+    if (both || !spaced || M <= 0 || N <= 0 || K <= 0 || few_in_registers(M, N, K, false) || !in_pieces(M, N, K)) return 0;
     return mxfp4_pieces_bytes(M, (K + MX_BLOCK - 1) / MX_BLOCK);
 }
 
@@ -56,8 +57,9 @@ TS_API int ts_gemm_mxfp4(const void* w_codes, const void* w_scales, long long w_
     if (M == 0) return 0;
     MxParams p{(const uint8_t*)w_codes, (const uint8_t*)w_scales, w_ld_codes, w_ld_scales, (const uint8_t*)x_scales, x_ld_scales, y, ldy,
                M, N, K, blocks, N / 2, out_dtype == TS_F32 ? 1 : 0, act, limit, alpha, 0, nullptr, 0, settled, 1, error};
-    const long long pieces = ts_gemm_mxfp4_scratch_bytes(M, N, K, x_scales != nullptr);
-    if (pieces && mxfp4_takes_pieces(w_codes, w_ld_codes, K)) {
+    const int spaced = (uintptr_t)w_codes % 32 == 0 && w_ld_codes % 32 == 0;
+    const long long pieces = ts_gemm_mxfp4_scratch_bytes(M, N, K, x_scales != nullptr, spaced);
+    if (pieces) {
         TS_REQUIRE(scratch && (uintptr_t)scratch % 16 == 0, "gemm_mxfp4: %lld bytes of scratch are needed", pieces);
         return mxfp4_pieces(x, ldx, scratch, p, gated, stream);
     }

@@ -42,7 +42,6 @@ struct MxParams {
 int mxfp4_rows16(const void* x, long long ldx, MxParams& p, int gated, cudaStream_t stream);
 int mxfp4_rows4(const void* x, long long ldx, MxParams& p, int gated, cudaStream_t stream);
 // A few rows in bfloat16, 64 at most, as three pieces of eight bits, which take `scratch`.
-bool mxfp4_takes_pieces(const void* w_codes, long long w_ld_codes, int K);
 long long mxfp4_pieces_bytes(int M, int blocks);
 int mxfp4_pieces(const void* x, long long ldx, void* scratch, MxParams& p, int gated, cudaStream_t stream);
 

@@ -538,10 +538,6 @@ int mxfp4_rows4(const void* x, long long ldx, MxParams& p, int gated, cudaStream
     return gated ? dispatch<true>(x, ldx, p, stream) : dispatch<false>(x, ldx, p, stream);
 }
 
-bool mxfp4_takes_pieces(const void* w_codes, long long w_ld_codes, int K) {
-    return K % 128 == 0 && w_ld_codes % 32 == 0 && (uintptr_t)w_codes % 32 == 0;      // what TMA asks of 4-bit numbers that it spaces out
-}
-
 long long mxfp4_pieces_bytes(int M, int blocks) { return (long long)M * PIECES8 * (blocks * 32ll + (blocks + 15) / 16 * 16); }
 
 int mxfp4_pieces(const void* x, long long ldx, void* scratch, MxParams& p, int gated, cudaStream_t stream) {

@@ -111,7 +111,7 @@ _SIGNATURES = {
     "ts_quantize_mxfp4": ("int", "ppplilllip"),
     "ts_dequantize_mxfp4": ("int", "ppplillip"),
     "ts_gemm_mxfp4": ("int", "ppllplplp" "iiil" "iiffipipp"),
-    "ts_gemm_mxfp4_scratch_bytes": ("long long", "iiii"),
+    "ts_gemm_mxfp4_scratch_bytes": ("long long", "iiiii"),
 }
 _CTYPES = {"p": ctypes.c_void_p, "i": ctypes.c_int, "l": ctypes.c_longlong, "f": ctypes.c_float}
 _RETURNS = {"int": ctypes.c_int, "long long": ctypes.c_longlong, "void": None, "const char*": ctypes.c_char_p}
@@ -227,7 +227,7 @@ class Ops:
         # TINYSERVE_B200_TILES=0 keeps the recurrences that have a form of sixteen tokens at a time on the scan token by token
         self.recurrence_tiles = os.environ.get("TINYSERVE_B200_TILES", "1") != "0"
         self._tile_floats: dict[tuple[int, int, int, int], tuple[int, int]] = {}   # sizes of a tile's buffers
-        self._scratch_mxfp4: dict[tuple[int, int, int], int] = {}                   # bytes of scratch of a product over 4-bit weights
+        self._scratch_mxfp4: dict[tuple[int, int, int, bool], int] = {}             # bytes of scratch of a product over 4-bit weights
         # TINYSERVE_B200_OVERLAP=0 keeps a replayed step's kernels on one stream (see parts/overlap.py)
         self.overlap = os.environ.get("TINYSERVE_B200_OVERLAP", "1") != "0"
         # TINYSERVE_B200_LRU=split keeps a gated linear recurrent unit's decode steps on the kernels of prompt portions
@@ -1769,18 +1769,19 @@ class Ops:
                 raise KernelError(f"{who}: out is {tuple(out.shape)}, the product {(M, cols)}")
         if M == 0 or cols == 0:
             return out
-        scratch = None
+        scratch, codes = None, w.codes.data_ptr()
         if not both:
-            size = self._scratch_mxfp4.get((M, N, K))
+            spaced = (codes | w.ld_codes) % 32 == 0          # rows of codes as the product in pieces takes them
+            size = self._scratch_mxfp4.get((M, N, K, spaced))
             if size is None:
-                size = int(self.lib.ts_gemm_mxfp4_scratch_bytes(M, N, K, 0))
+                size = int(self.lib.ts_gemm_mxfp4_scratch_bytes(M, N, K, 0, spaced))
                 if M <= 64:                                  # the sizes of decode steps come again and again
-                    self._scratch_mxfp4[(M, N, K)] = size
+                    self._scratch_mxfp4[(M, N, K, spaced)] = size
             if size:
                 scratch = torch.empty((size,), dtype=torch.uint8, device=rows.device)
                 self.launches += 1                           # the kernel that takes x apart
         gated, kind = (0, 0) if activation is None else (1, self.GATED_ACTIVATIONS[activation])
-        self._call("ts_gemm_mxfp4", w.codes.data_ptr(), w.scales.data_ptr(), w.ld_codes, w.ld_scales, rows.data_ptr(), ldx, x_scales, x_ld_scales,
+        self._call("ts_gemm_mxfp4", codes, w.scales.data_ptr(), w.ld_codes, w.ld_scales, rows.data_ptr(), ldx, x_scales, x_ld_scales,
                    out.data_ptr(), M, N, K, cols, gated, kind, limit, alpha, w.settled, _ptr(scratch), _DTYPE_CODE[out_dtype],
                    self.error_word().data_ptr(), _stream())
         return out
