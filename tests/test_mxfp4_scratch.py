@@ -116,3 +116,21 @@ def test_scratch_on_two_streams(ops, weight):
     for a, results in zip(alone, found):
         assert all(torch.equal(a, r) for r in results)
     ops.check_device_errors()
+
+
+def test_what_is_no_matrix_in_four_bits_is_refused():
+    """A bfloat16 weight, or one's codes alone, where an MXFP4 is wanted; a class derived from it is one."""
+    from tinyserve_llm_b200.ops import KernelError, Ops
+    ops, x = Ops.__new__(Ops), torch.zeros((4, 64), dtype=torch.bfloat16)
+    for call in (lambda w: ops.linear_mxfp4(x, w), lambda w: ops.linear_gated_mxfp4(x, w, "silu"), ops.dequantize_mxfp4):
+        for bad in (x, None, torch.zeros((4, 32), dtype=torch.uint8)):
+            with pytest.raises(KernelError, match="MXFP4"):
+                call(bad)
+
+    class Derived(MXFP4):
+        pass
+
+    q = Derived(torch.zeros((4, 32), dtype=torch.uint8), torch.zeros((4, 16), dtype=torch.uint8)[:, :2], 64)
+    other = MXFP4(torch.zeros((4, 16), dtype=torch.uint8), torch.zeros((4, 16), dtype=torch.uint8)[:, :1], 32)
+    with pytest.raises(KernelError, match=r"x is \(4, 64\), the weight has rows of 32"):
+        ops.linear_mxfp4(q, other)

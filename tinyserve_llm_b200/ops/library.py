@@ -1700,8 +1700,8 @@ class Ops:
 
     def dequantize_mxfp4(self, q: MXFP4, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
         """The numbers q stands for, [rows, cols] in bfloat16 or float32: exact, but for what the type has no room for (infinite)."""
-        if dtype not in _DTYPE_CODE:
-            raise KernelError(f"dequantize_mxfp4: dtype {dtype}, expected one of {tuple(_DTYPE_CODE)}")
+        if not isinstance(q, MXFP4) or dtype not in _DTYPE_CODE:
+            raise KernelError(f"dequantize_mxfp4: {type(q).__name__} to {dtype}; an MXFP4 goes to one of {tuple(_DTYPE_CODE)}")
         self._check_here(q.codes, "q")
         out = torch.empty((q.rows, q.cols), dtype=dtype, device=q.device)
         if q.rows:
@@ -1728,6 +1728,8 @@ class Ops:
         act(x . Wgate^T, x . Wup^T), bfloat16 [M, I], for the activations of `gated_activation` and x as `linear_mxfp4` takes it; Wgate and
         Wup are the two halves of the weight's rows.  The activation reads the float32 sums: one rounding, at the end.
         """
+        if not isinstance(gate_up_weight, MXFP4):
+            raise KernelError(f"linear_gated_mxfp4: the weight must be an MXFP4, got {type(gate_up_weight).__name__}")
         if gate_up_weight.rows % 2 or activation not in self.GATED_ACTIVATIONS:
             raise KernelError(f"linear_gated_mxfp4: the weight must hold gate and up halves ({gate_up_weight.rows} rows); activation "
                               f"{activation!r} of {sorted(self.GATED_ACTIVATIONS)}")
@@ -1735,8 +1737,10 @@ class Ops:
 
     def _product_mxfp4(self, who: str, x: torch.Tensor | MXFP4, w: MXFP4, activation: str | None, limit: float, alpha: float,
                        out_dtype: torch.dtype, out: torch.Tensor | None) -> torch.Tensor:
+        if not isinstance(w, MXFP4):
+            raise KernelError(f"{who}: the weight must be an MXFP4, got {type(w).__name__}")
         M, K, N = -1, -1, w.rows
-        both = type(x) is MXFP4
+        both = isinstance(x, MXFP4)
         if both:
             M, K, rows, ldx, x_scales, x_ld_scales = x.rows, x.cols, x.codes, x.ld_codes, x.scales.data_ptr(), x.ld_scales
         else:
