@@ -90,8 +90,8 @@ def test_small_numbers_beside_large_ones(ops, m, n, k, every):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("m, inter, k", [(3, 256, 512), (8, 4200, 2048), (9, 6000, 512), (24, 4800, 1792), (64, 1301, 2048), (40, 2600, 4096), (33, 9601, 4096),
-                                         (200, 4700, 640), (100, 150, 512)])
+@pytest.mark.parametrize("m, inter, k", [(3, 256, 512), (8, 4200, 2048), (9, 6000, 512), (24, 4800, 1792), (64, 1301, 2048), (40, 2600, 4096),
+                                         (33, 9601, 4096), (200, 4700, 640), (100, 150, 512)])
 def test_gated_small_numbers_beside_large_ones(ops, m, inter, k):
     x, column = far_apart(m, k, 3, m + k)
     weight, values = weights(2 * inter, k, column, inter + k)
@@ -133,3 +133,29 @@ def test_the_largest_numbers(ops, m, n, k):
     at = 37 + np.arange(n) % 3
     got = f64(ops.linear_mxfp4(x.to(DEV), one_a_row(n, k, at, 2), out_dtype=torch.float32))
     np.testing.assert_array_equal(got, f64(x)[:, at])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m, n, k", [(1, 9000, 2048), (2, 1300, 16384), (12, 1300, 4224), (30, 1300, 4224), (33, 5200, 4096), (9, 130, 65536)])
+def test_stretches_of_wider_rows(ops, m, n, k):
+    """Rows of x apart from one another, one of them with infinities and one with a NaN: each row gives what it gives by itself, in a row of its own."""
+    x, column = far_apart(m, k, 5, 3)
+    if m > 2:
+        x[0, 70], x[0, k - 1], x[2, 40] = float("inf"), float("-inf"), float("nan")
+    weight, values = weights(n, k, column, n + k)
+    wide = torch.full((m, k + 72), float("nan"), dtype=torch.bfloat16)
+    wide[:, 64:64 + k] = x
+    part = wide.to(DEV)[:, 64:64 + k]
+    assert part.stride(0) == k + 72 and part.data_ptr() % 16 == 0
+    got = ops.linear_mxfp4(part, weight, out_dtype=torch.float32)
+    assert torch.equal(got.nan_to_num(nan=7.0), ops.linear_mxfp4(x.to(DEV), weight, out_dtype=torch.float32).nan_to_num(nan=7.0))
+    xv = f64(x)
+    with np.errstate(invalid="ignore"):
+        want = xv @ values.T
+    np.testing.assert_array_equal(np.isnan(f64(got)), np.isnan(want))
+    infinite = np.isinf(want)
+    np.testing.assert_array_equal(f64(got)[infinite], want[infinite])
+    finite = np.isfinite(xv).all(axis=1)
+    check(got[torch.from_numpy(finite).to(DEV)], want[finite], bound(xv[finite], values, k))
+    torch.cuda.synchronize()
+    ops.check_device_errors()

@@ -3,9 +3,10 @@
 #include "skinny_mxfp4.h"
 
 // Whether a few rows go by the kernel that spreads codes in registers: no kernel has less between its launch and its end, but it takes a
-// cycle for every 13 numbers of W and SM.  Measured on a B200 (graphs of different weights): 2,048 by 2,048, 1 to 16 rows in bfloat16 2.9 to
-// 4.1 us (in pieces 7.2 to 8.0), in four bits 3.1 to 3.7 (tcgen05 4.4 to 5.1); 2,048 by 8,192, 1 to 8 rows in bfloat16 8.1 to 9.0 (9.2 to
-// 10.0), 16 rows 11.7 (10.2); 16,384 by 2,048, 8 rows 13.2 (10.7).
+// cycle for every 13 numbers of W and SM.  Device times on a B200 (graphs of different weights): 2,048 by 2,048, 1 to 16 rows in bfloat16 2.9
+// to 4.2 us (in pieces 7.4 to 8.1), in four bits 3.1 to 3.7 (tcgen05 4.4 to 5.1); 2,048 by 8,192, 1 to 8 rows in bfloat16 8.1 to 9.0 (9.9 to
+// 10.3), 16 rows 11.7 (11.0); 4,096 by 4,096 7.9 to 8.8 (8.4 to 8.9), 16 rows 11.2 (9.3); 6,144 by 4,096 10.6 to 11.7 (10.3 to 10.7); 16,384 by
+// 2,048 11.1 to 13.2 (10.6 to 10.8).
 static bool few_in_registers(int M, int N, int K, bool both) {
     const long long numbers = (long long)N * K;
     return (M <= SKINNY_MX_ROWS && numbers <= 5ll << 20) || (!both && M <= 8 && numbers <= 1ll << 24);

@@ -9,7 +9,8 @@
 //
 // Many tiles: persistent, one CTA an SM, with two accumulators, so that a tile's epilogue runs under the next one's MMAs, or one of 256 columns,
 // beside whose epilogue the next tile's operands are made.  Few tiles: a cluster of `splits` CTAs takes a tile, each its share of K, and leaves
-// its sums in its own shared memory; each CTA then adds up a share of the columns from all of them, in the order of their ranks.  Nothing of that needs a workspace in global memory, and the order is fixed.
+// its sums in its own shared memory; each CTA then adds up a share of the columns from all of them, in the order of their ranks.  Nothing of
+// that needs a workspace in global memory, and the order is fixed.
 //
 // Every wait on an mbarrier gives up after about two seconds, records where in an error word the host can read, and the CTA goes on to
 // free its tensor memory and return.

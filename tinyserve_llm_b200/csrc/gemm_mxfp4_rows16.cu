@@ -7,8 +7,9 @@
 //
 // Bound by instructions: some 1,900 of a warp for 64 columns of K and a tile, half of them the codes' (27 for a warp's 8 x 32 codes), at 0.64 of the
 // issue slots, tensor cores 0.67 busy.  So tiles are as wide as tensor memory lets them be, 256 rows of x on one accumulator: codes once spread
-// serve 256 columns, and a tile's epilogue costs less than it would save to hide it.  Gated 2,048 rows over 2 x 8,192 by 2,048 115 us with 192 rows and two accumulators, 106 with
-// 256 and one (1.30 PFLOP/s); 2,048 rows through an 8B model's gate and up projections 376 and 344 (1.40).
+// serve 256 columns, and a tile's epilogue costs less than it would save to hide it.  Device times in a graph: gated, 2,048 rows over 2 x 8,192
+// by 2,048, 115 us with 192 rows and two accumulators, 104 to 106 with 256 and one (1.30 PFLOP/s; a call from Python takes 125); 2,048 rows
+// through an 8B model's gate and up projections 376 and 344 (1.40).
 #include "gemm_mxfp4.cuh"
 
 namespace {

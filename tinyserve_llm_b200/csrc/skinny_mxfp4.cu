@@ -8,11 +8,13 @@
 // Every thread owns a ring of slots in shared memory for its own blocks, filled by cp.async, so the copies in flight are bounded by shared
 // memory and there is no barrier.  Weights written long ago (`settled`) are asked for before the wait for the kernel ahead on the stream.
 //
-// Bound by instructions, not by memory: a unit's 1,088 bytes of W take 330 of a warp, 200 of them to spread its codes, where HBM brings them in
-// the time of 190; with eight rows x's loads, 16 bytes a thread of 64-byte pieces, keep L1 busy too (28,672 by 4,096, eight rows: 41 us, L1 0.85
-// busy, ALU 0.44).  What it has is the least between launch and end: 2,048 by 2,048, one row, 2.9 us (2.3 where W was written long ago).
+// Not bound by memory: a unit's 1,088 bytes of W take 330 instructions of a warp, 200 of them to spread its codes, where HBM brings them in the
+// time of 190, and x's loads, 16 bytes a thread of 64-byte pieces, keep L1 busy (2,048 by 8,192, eight rows: 9.0 us, 7.5 where W was written
+// long ago; L1 0.64 busy, a third of the issue slots, DRAM 0.09).  What it has is the least between launch and end: 2,048 by 2,048, one row,
+// 3.0 us (2.4).
 //
-// The split of K depends on N and K only, never on the number of rows of x, so a row's result does not depend on what else is in the batch.
+// The split of K depends on N and K only, so among the calls that come here a row's result does not depend on the rows beside it.  Which kernel a
+// call takes does depend on their number (gemm_mxfp4.cu: it changes behind 8, 16, 32 and 64 rows), and another kernel adds in another order.
 #include "mxfp4.cuh"
 #include "skinny_mxfp4.h"
 
